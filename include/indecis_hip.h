@@ -386,6 +386,130 @@ int ixh_attend8(int device, float *o, const float *q, const float *k,
                 const float *v, int n, int d, int window, float scale,
                 int lanes);
 
+/* ---- float attention on device rows -------------------------------------- */
+
+/* Attention and the norms of queries and keys of encoders and prefix models
+ * whose layers are not the reference's: float rows in device memory, forward
+ * and backward (no counterpart in the reference, whose int8 attention is
+ * ixh_attend8). Every call queues its work on `stream` (a hipStream_t; NULL:
+ * the null stream) of GPU `device` and returns without waiting; it allocates
+ * nothing and may be captured into a graph. What a call needs beside its
+ * arguments it takes from the caller's workspace, which no other call may
+ * use until this one's work is done. Offsets, positions, documents and
+ * buckets are read on the device and never checked on the host: values out
+ * of range read and write nothing out of range. Rows before offs[0] and from
+ * offs[B] on are neither read nor written. Outputs may not overlap inputs
+ * unless said otherwise. Results do not depend on the run: no sum's order
+ * changes from one call to the next. */
+enum { IXH_TYPE_F32 = 0, IXH_TYPE_BF16 = 1, IXH_TYPE_F16 = 2 };
+
+/* Rows of heads in device memory: value i of a head of a row stands at
+ * p[row * r + head * h + i], in values of the call's type. p and both
+ * strides are multiples of 16 bytes. */
+typedef struct ixh_heads {
+  void *p;
+  int64_t row, head;
+} ixh_heads;
+
+typedef struct ixh_attend_args {
+  int type;              /* IXH_TYPE_* of q, k, v, o and table */
+  int B;                 /* sequences */
+  int nq, nk;            /* rows of the packed queries and keys, at most 2^30 */
+  int heads, kv_heads;   /* heads % kv_heads == 0: head h reads key head h / (heads / kv_heads) */
+  int dim;               /* of a head, a multiple of 8 up to 128 */
+  ixh_heads q, k, v, o;  /* [nq][heads][dim], [nk][kv_heads][dim] twice, [nq][heads][dim] */
+  const int32_t *q_offs; /* [B+1]: rows of each sequence's queries, ascending */
+  const int32_t *k_offs; /* [B+1] of its keys; NULL: q_offs, and nk == nq */
+  float scale;           /* of the products, > 0 */
+  float cap;             /* > 0: scores become cap * tanh(score / cap); 0: not */
+  const float *slopes;   /* [heads]: score -= slope * distance; NULL: none */
+  const void *table;     /* [n_buckets][heads]: score += table[bucket][head]; NULL: none */
+  const int32_t *buckets; /* [2 reach + 1]: the bucket of distance -reach..reach (key less
+                             query), those further off taken as the ends; not in
+                             0..n_buckets-1: no bias there */
+  int n_buckets, reach;  /* reach in 1..1024, n_buckets in 1..65536 */
+  const int32_t *q_docs; /* [nq]: a query sees the keys of its own document; < 0: nothing
+                            (padding); NULL: all of its sequence */
+  const int32_t *k_docs; /* [nk]; NULL: q_docs, and nk == nq */
+  int causal;            /* a query sees no later key */
+  const int32_t *prefix; /* [B], with causal: but every query the first prefix[b] keys */
+  int window;            /* >= 0: only keys at most this far off; < 0: any */
+  float *lse;            /* [heads][nq]: log of the sum of exp(score); -inf where a query
+                            sees nothing. Written by the forward if not NULL, read by
+                            the backward */
+  void *workspace;       /* ixh_attend_workspace bytes, 16-byte aligned */
+  int64_t workspace_bytes;
+} ixh_attend_args;
+
+/* What ixh_attend_backward writes (d_out is read); dtable [n_buckets][heads]
+ * of the call's type, or NULL. */
+typedef struct ixh_attend_grads {
+  ixh_heads d_out, dq, dk, dv;
+  void *dtable;
+} ixh_attend_grads;
+
+/* Bytes of workspace that a call with these sizes takes (0: none needed). */
+int ixh_attend_workspace(const ixh_attend_args *a, int backward, int64_t *bytes);
+/* o = softmax(scores) v over each query's visible keys. A sequence's last
+ * query stands at its last key (a single new query attends over all keys
+ * given); distances and the causal mask go by these places. Sums and
+ * statistics are 32-bit; the probabilities are rounded to the rows' type
+ * before the second product. A query that sees nothing gets o = 0. A key
+ * whose document is < 0 may hold anything; other masked keys must be
+ * finite, as a product with probability 0 reads them. */
+int ixh_attend(int device, const ixh_attend_args *a, void *stream);
+/* The gradients of ixh_attend at the same arguments, o and lse as it left
+ * them: dq, dk (over the heads that share it), dv, and the table's. */
+int ixh_attend_backward(int device, const ixh_attend_args *a, const ixh_attend_grads *g, void *stream);
+
+/* The buckets of a learned distance bias, map [2 max_distance + 1] for
+ * distances -max_distance..max_distance (key less query): one bucket a
+ * distance up to half of a direction's buckets, then on a logarithmic scale
+ * up to max_distance, its borders compared exactly in whole numbers.
+ * bidirectional: half of the buckets for later keys, else these share bucket
+ * 0. buckets even (bidirectional) and at least 4 (2) and at most 1024,
+ * max_distance over a direction's linear buckets and at most 1024. Host
+ * only. */
+int ixh_rel_buckets(int buckets, int max_distance, int bidirectional, int32_t *map);
+
+enum { IXH_HEAD_NORM_NONE = 0, IXH_HEAD_NORM_RMS = 1, IXH_HEAD_NORM_LAYER = 2 };
+enum { IXH_PAIRS_HALVES = 0, IXH_PAIRS_NEIGHBOURS = 1 };
+
+typedef struct ixh_norm_rope_args {
+  int type;                    /* of the rows */
+  int n, q_heads, k_heads, dim; /* dim a multiple of 8 up to 256; either head count may be 0 */
+  ixh_heads q, k;              /* [n][q_heads][dim], [n][k_heads][dim] */
+  ixh_heads q_out, k_out;      /* may be q and k themselves */
+  int norm;                    /* IXH_HEAD_NORM_*: x / sqrt(mean x^2 + eps), LAYER with the
+                                  mean taken off first; then times gamma */
+  double eps;
+  int gamma_type;              /* IXH_TYPE_F32 or the rows' type */
+  const void *q_gamma, *k_gamma; /* [dim]; NULL: ones */
+  const float *cos, *sin;      /* [rows][rot / 2] */
+  int rows, rot;               /* the first rot columns are rotated: a multiple of 16 for
+                                  halves (i with i + rot / 2, as the reference's Rope),
+                                  even for neighbours (2i with 2i + 1); 0: none */
+  int pairs;                   /* IXH_PAIRS_* */
+  const int32_t *pos;          /* [n]: row of cos and sin; NULL: the row itself. A place
+                                  outside them gives NaN in the rotated columns */
+  void *workspace;             /* the backward's */
+  int64_t workspace_bytes;
+} ixh_norm_rope_args;
+
+/* d*_out are read; dq and dk (which may be dq_out and dk_out) and the gammas'
+ * gradients (of gamma_type; NULL: not wanted) are written. */
+typedef struct ixh_norm_rope_grads {
+  ixh_heads dq_out, dk_out, dq, dk;
+  void *dq_gamma, *dk_gamma;
+} ixh_norm_rope_grads;
+
+/* The norm of each head's row and the rotation of its first columns, for Q
+ * and K in one launch; 32-bit arithmetic, one rounding. */
+int ixh_qk_norm_rope(int device, const ixh_norm_rope_args *a, void *stream);
+int ixh_qk_norm_rope_workspace(const ixh_norm_rope_args *a, int64_t *bytes);
+/* Its gradients, from the inputs q and k (q_out and k_out are not used). */
+int ixh_qk_norm_rope_backward(int device, const ixh_norm_rope_args *a, const ixh_norm_rope_grads *g, void *stream);
+
 /* Self-check of the attention kernels' softmax rounding (no counterpart in
  * the reference; for tests and deployment checks). The kernels round
  * 255*exp(s - max) with the device's base-2 exponential and fall back to

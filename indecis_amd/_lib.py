@@ -27,6 +27,8 @@ EXPORTS = [
     "ixh_check_exp255", "ixh_check_gelu", "ixh_check_mfma_rate", "ixh_batcher_create", "ixh_batcher_encode", "ixh_batcher_stats",
     "ixh_batcher_destroy", "ixh_model_set_option", "ixh_model_get_option", "ixh_packb8_set_option",
     "ixh_model_set_heads", "ixh_encode_heads", "ixh_matmul8_noalloc",
+    "ixh_attend", "ixh_attend_backward", "ixh_attend_workspace", "ixh_rel_buckets", "ixh_qk_norm_rope",
+    "ixh_qk_norm_rope_backward", "ixh_qk_norm_rope_workspace",
 ]
 
 IXH_OK, IXH_EINVAL, IXH_ERANGE, IXH_ESTATE, IXH_EHIP, IXH_ENOMEM, IXH_EFORMAT = range(7)
@@ -35,6 +37,9 @@ MAT_QKV, MAT_O, MAT_I, MAT_OMLP = range(4)
 NORM_EMB, NORM_ATTN, NORM_MLP, NORM_FINAL = range(4)
 LAYOUT_ROWS, LAYOUT_PANELS = 0, 1
 OUT_POOLED, OUT_TOKENS = 0, 1
+TYPE_F32, TYPE_BF16, TYPE_F16 = range(3)
+HEAD_NORMS = {"none": 0, "rms": 1, "layer": 2}
+PAIRS = {"halves": 0, "neighbours": 1}
 (OPT_PARTS, OPT_PASS_TOKENS, OPT_QKV_FUSED, OPT_QKV_HEADS, OPT_GEMM, OPT_GEMM_TILE,
  OPT_LN_SEG, OPT_FUSE_RES, OPT_FUSE_MLP, OPT_QKV_KBLOCK, OPT_FEW_ROWS) = range(11)
 OPTIONS = {"parts": OPT_PARTS, "pass_tokens": OPT_PASS_TOKENS, "qkv_fused": OPT_QKV_FUSED,
@@ -64,8 +69,44 @@ class IxhConfig(C.Structure):
     ]
 
 
-_lib = None
 vp = C.c_void_p
+
+
+class IxhHeads(C.Structure):
+    _fields_ = [("p", vp), ("row", C.c_int64), ("head", C.c_int64)]
+
+
+class IxhAttendArgs(C.Structure):
+    _fields_ = [
+        ("type", C.c_int), ("B", C.c_int), ("nq", C.c_int), ("nk", C.c_int), ("heads", C.c_int),
+        ("kv_heads", C.c_int), ("dim", C.c_int), ("q", IxhHeads), ("k", IxhHeads), ("v", IxhHeads),
+        ("o", IxhHeads), ("q_offs", vp), ("k_offs", vp), ("scale", C.c_float), ("cap", C.c_float),
+        ("slopes", vp), ("table", vp), ("buckets", vp), ("n_buckets", C.c_int), ("reach", C.c_int),
+        ("q_docs", vp), ("k_docs", vp), ("causal", C.c_int), ("prefix", vp), ("window", C.c_int),
+        ("lse", vp), ("workspace", vp), ("workspace_bytes", C.c_int64),
+    ]
+
+
+class IxhAttendGrads(C.Structure):
+    _fields_ = [("d_out", IxhHeads), ("dq", IxhHeads), ("dk", IxhHeads), ("dv", IxhHeads), ("dtable", vp)]
+
+
+class IxhNormRopeArgs(C.Structure):
+    _fields_ = [
+        ("type", C.c_int), ("n", C.c_int), ("q_heads", C.c_int), ("k_heads", C.c_int), ("dim", C.c_int),
+        ("q", IxhHeads), ("k", IxhHeads), ("q_out", IxhHeads), ("k_out", IxhHeads), ("norm", C.c_int),
+        ("eps", C.c_double), ("gamma_type", C.c_int), ("q_gamma", vp), ("k_gamma", vp), ("cos", vp),
+        ("sin", vp), ("rows", C.c_int), ("rot", C.c_int), ("pairs", C.c_int), ("pos", vp),
+        ("workspace", vp), ("workspace_bytes", C.c_int64),
+    ]
+
+
+class IxhNormRopeGrads(C.Structure):
+    _fields_ = [("dq_out", IxhHeads), ("dk_out", IxhHeads), ("dq", IxhHeads), ("dk", IxhHeads),
+                ("dq_gamma", vp), ("dk_gamma", vp)]
+
+
+_lib = None
 
 
 def lib():
@@ -128,6 +169,13 @@ def lib():
         "ixh_packb8_set_option": [vp, C.c_int, C.c_int64],
         "ixh_model_set_heads": [vp, C.c_int, vp, vp, vp, vp],
         "ixh_encode_heads": [vp, vp, vp, C.c_int, C.c_int, vp, vp],
+        "ixh_attend": [C.c_int, vp, vp],
+        "ixh_attend_backward": [C.c_int, vp, vp, vp],
+        "ixh_attend_workspace": [vp, C.c_int, C.POINTER(C.c_int64)],
+        "ixh_rel_buckets": [C.c_int, C.c_int, C.c_int, vp],
+        "ixh_qk_norm_rope": [C.c_int, vp, vp],
+        "ixh_qk_norm_rope_backward": [C.c_int, vp, vp, vp],
+        "ixh_qk_norm_rope_workspace": [vp, C.POINTER(C.c_int64)],
         "ixh_matmul8_noalloc": [vp, vp, C.c_int, vp, C.c_int, C.c_int, C.c_int, vp],
     }
     for name, args in sig.items():

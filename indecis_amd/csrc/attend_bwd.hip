@@ -1,0 +1,591 @@
+// attend_bwd.hip — the gradients of attend_fwd.hip, from the rows, the
+// output and the logarithms of the sums that the forward left.
+//
+// With P = 2^(z - lse) taken again, dP = dO V^T and delta = dO . o:
+//   dZ = P (dP - delta), dS = dZ z'(s),
+//   dQ = scale dS K, dK = scale dS^T Q, dV = P^T dO.
+// Two kernels, so that no sum crosses workgroups and no result depends on
+// an order of atomics: one has a block of queries and runs over the keys
+// (dQ, delta and the bias' sums), one has a block of keys and runs over
+// the queries of every head that shares them (dK, dV). Both take S and dP
+// again: 7 products for the 5 of one kernel with atomics.
+#include "attend_device.h"
+#include "ixh_internal.h"
+
+namespace ixh {
+namespace {
+
+// z and its derivative by the score where there is a cap, for 16 scores.
+template <class T, int FEAT>
+__device__ __forceinline__ void shape_scores(v16f &z, float *slope_of, const Score &sc) {
+#pragma unroll
+  for (int r = 0; r < 16; r++) {
+    if constexpr (FEAT & kCap) {
+      float u;
+      z[r] = sc.c2 * tanh_of<T>(z[r] * sc.c1, &u);
+      slope_of[r] = 4.0f * u * (1.0f - u);
+    } else {
+      z[r] *= sc.c1;
+    }
+  }
+}
+
+// ---- dQ ---------------------------------------------------------------------
+
+template <class T, int DT>
+struct DqShape {
+  static constexpr int WAVES = 4, THREADS = 256, ROWS = 128;
+  static constexpr int BK = 32;
+  typedef Tile<T, DT, BK, THREADS> KV;
+  static constexpr int DOCS = 4 * KV::BYTES, BIAS = DOCS + 2 * 4 * BK;
+};
+
+template <class T, int DT, int FEAT>
+__global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : 2) void attend_dq_kernel(AttendArgs x) {
+  typedef DqShape<T, DT> Sh;
+  typedef typename Sh::KV KV;
+  typedef typename Kind<T>::frag Frag;
+  constexpr int THREADS = Sh::THREADS, ROWS = Sh::ROWS, BK = Sh::BK, KS = DT / 16, ND = DT / 32;
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  const ixh_attend_args &a = x.a;
+  const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  int *const kdocs = (int *)(smem + Sh::DOCS);
+  float *const bias = (float *)(smem + Sh::BIAS);
+  // sums of dZ by distance, an array each half of a wave
+  const int span = 2 * a.reach + 1;
+  float *const dist = bias + attend_bias_len(a.reach);
+
+  const int head = blockIdx.x % a.heads, kvh = head / x.group;
+  const int64_t slot = x.slots - 1 - blockIdx.x / a.heads;
+  int b;
+  int64_t blk;
+  find_block(a.q_offs, a.B, a.nq, ROWS, 1, slot, &b, &blk);
+  const Seq s(a, b);
+  const bool grad_table = (FEAT & kBias) && x.dist;
+  float *const dist_out = grad_table ? x.dist + (slot * a.heads + head) * span : nullptr;
+  if (blk * ROWS >= s.nq) {
+    if (grad_table)
+      for (int i = tid; i < span; i += THREADS) dist_out[i] = 0.0f;
+    return;
+  }
+  const int first = (int)(blk * ROWS);
+  const int tok = min(first + wave * 32 + (lane & 31), s.nq - 1);
+  const bool mine = first + wave * 32 + (lane & 31) < s.nq;
+  const int p = tok + s.shift;
+  int lo, hi;
+  key_bounds(a, s, p, &lo, &hi);
+  const int p_lo = __builtin_amdgcn_readlane(p, 0), p_hi = __builtin_amdgcn_readlane(p, 31);
+  const int lo_min = __builtin_amdgcn_readlane(lo, 0), lo_max = __builtin_amdgcn_readlane(lo, 31);
+  const int hi_min = __builtin_amdgcn_readlane(hi, 0), hi_max = __builtin_amdgcn_readlane(hi, 31);
+  if (hi < lo) lo = 1 << 30, hi = 1 << 30;
+  const unsigned width = hi - lo;
+  int t_begin, t_end;
+  {
+    int l, u, unused;
+    key_bounds(a, s, first + s.shift, &l, &unused);
+    key_bounds(a, s, min(first + ROWS, s.nq) - 1 + s.shift, &unused, &u);
+    t_begin = l / BK;
+    t_end = u >= l ? u / BK + 1 : t_begin;
+  }
+  const int64_t row = s.q0 + tok;
+  const int doc = a.q_docs ? max(a.q_docs[row], -1) : 0;
+
+  // a row that sees nothing has lse -inf: its dO and o are not read
+  const float lse = a.lse[(int64_t)head * a.nq + row];
+  const bool alive = lse > -INFINITY;
+  const float lse2 = alive ? lse * kLog2e : 0.0f;
+  Frag q[KS], dO[KS];
+  float delta = 0.0f;
+  {
+    const T *qr = (const T *)a.q.p + row * a.q.row + head * a.q.head;
+    const T *gr = (const T *)x.g.d_out.p + row * x.g.d_out.row + head * x.g.d_out.head;
+    const T *orow = (const T *)a.o.p + row * a.o.row + head * a.o.head;
+#pragma unroll
+    for (int i = 0; i < KS; i++) {
+      const bool in = 16 * i + 8 * h < a.dim && alive;
+      q[i] = load8(qr + 16 * i + 8 * h, in);
+      dO[i] = load8(gr + 16 * i + 8 * h, in);
+      const Frag o = load8(orow + 16 * i + 8 * h, in);
+#pragma unroll
+      for (int e = 0; e < 8; e++) delta = __builtin_fmaf(frag_at(dO[i], e), frag_at(o, e), delta);
+    }
+    delta = half_sum(delta);
+    if (mine && h == 0) x.delta[(int64_t)head * a.nq + row] = delta;
+  }
+  const T *const kb = (const T *)a.k.p + s.k0 * a.k.row + kvh * a.k.head;
+  const T *const vb = (const T *)a.v.p + s.k0 * a.v.row + kvh * a.v.head;
+  const Score sc(a, FEAT & kCap);
+  const float slope = (FEAT & kBias) && a.slopes ? -a.slopes[head] * kLog2e : 0.0f;
+  if constexpr (FEAT & kBias) {
+    if (a.table) load_bias<T>(a, head, bias, tid, THREADS);
+    if (grad_table)
+      for (int i = tid; i < 2 * Sh::WAVES * span; i += THREADS) dist[i] = 0.0f;
+    __syncthreads();
+  }
+  float *const my_dist = dist + (2 * wave + h) * span;
+  float below = 0.0f, above = 0.0f;  // dZ at distances of -reach and less, reach and more
+
+  v16f acc[ND];
+#pragma unroll
+  for (int d = 0; d < ND; d++) acc[d] = v16f{};
+
+  KV kt, vt;
+  int kdoc = 0;
+  auto fetch = [&](int t) {
+    kt.get(kb, a.k.row, t * BK, s.nk, a.dim, tid);
+    vt.get(vb, a.v.row, t * BK, s.nk, a.dim, tid);
+    if (a.q_docs && tid < BK) kdoc = t * BK + tid < s.nk ? a.k_docs[s.k0 + t * BK + tid] : -1;
+  };
+  int buf = 0;
+  if (t_begin < t_end) fetch(t_begin);
+  for (int t = t_begin; t < t_end; t++, buf ^= 1) {
+    char *const kl = smem + buf * 2 * KV::BYTES, *const vl = kl + KV::BYTES;
+    const bool docs = a.q_docs != nullptr;
+    {
+      const bool all = a.dim == DT && t * BK + BK <= s.nk && !docs;
+      if (docs) {
+        if (tid < BK) kdocs[buf * BK + tid] = kdoc < 0 ? -2 : kdoc;
+        __syncthreads();
+      }
+      auto keep = [&](int r) { return t * BK + r < s.nk && (!docs || kdocs[buf * BK + r] >= 0); };
+      kt.put(kl, a.dim, tid, all, keep);
+      vt.put(vl, a.dim, tid, all, keep);
+    }
+    __syncthreads();
+    if (t + 1 < t_end) fetch(t + 1);
+    const int j0 = t * BK;
+    if (j0 > hi_max || j0 + BK <= lo_min) continue;
+
+    v16f z = v16f{}, dp = v16f{};
+#pragma unroll
+    for (int i = 0; i < KS; i++) {
+      z = mfma16(KV::rows(kl, 0, i, lane), q[i], z);
+      dp = mfma16(KV::rows(vl, 0, i, lane), dO[i], dp);
+    }
+    float by_cap[16];
+    shape_scores<T, FEAT>(z, by_cap, sc);
+    const int d0 = j0 + 4 * h - p;
+    const int near = j0 - p_hi, far = j0 + 31 - p_lo;
+    const bool flat = near >= a.reach || far <= -a.reach;
+    if constexpr (FEAT & kBias) {
+      if (a.slopes) {
+        const float f = (float)d0;
+#pragma unroll
+        for (int r = 0; r < 16; r++)
+          z[r] = __builtin_fmaf(slope, __builtin_fabsf(f + (float)(8 * (r >> 2) + (r & 3))), z[r]);
+      }
+      if (a.table) {
+        if (flat) {
+          const float c = bias[near >= a.reach ? 2 * (a.reach + kBiasPad) : 0];
+#pragma unroll
+          for (int r = 0; r < 16; r++) z[r] += c;
+        } else {
+          const float *at = bias + d0 + a.reach + kBiasPad;
+#pragma unroll
+          for (int r = 0; r < 16; r++) z[r] += at[8 * (r >> 2) + (r & 3)];
+        }
+      }
+    }
+    float dz[16];
+#pragma unroll
+    for (int r = 0; r < 16; r++) dz[r] = exp2_fast(z[r] - lse2) * (dp[r] - delta);
+    if (docs || j0 < lo_max || j0 + BK - 1 > hi_min || __ballot(!alive) != 0) {
+      const unsigned e0 = j0 + 4 * h - lo;
+#pragma unroll
+      for (int r = 0; r < 16; r++)
+        if (!alive || e0 + (unsigned)(8 * (r >> 2) + (r & 3)) > width) dz[r] = 0.0f;
+      if (docs) {
+#pragma unroll
+        for (int g = 0; g < 4; g++) {
+          const i4 d = *(const i4 *)(kdocs + buf * BK + 8 * g + 4 * h);
+#pragma unroll
+          for (int e = 0; e < 4; e++)
+            if (d[e] != doc) dz[4 * g + e] = 0.0f;
+        }
+      }
+    }
+    if constexpr (FEAT & kBias) {
+      if (grad_table && mine) {
+        if (flat) {
+          float part = 0.0f;
+#pragma unroll
+          for (int r = 0; r < 16; r++) part += dz[r];
+          if (near >= a.reach)
+            above += part;
+          else
+            below += part;
+        } else {
+          // register by register: the 32 queries of a half have 32 distances
+          // to one key, so no two lanes add to one place, and a wave's adds
+          // to its own arrays keep their order
+#pragma unroll
+          for (int r = 0; r < 16; r++) {
+            const int d = d0 + 8 * (r >> 2) + (r & 3);
+            if (d >= a.reach)
+              above += dz[r];
+            else if (d <= -a.reach)
+              below += dz[r];
+            else
+              __builtin_amdgcn_ds_faddf((__attribute__((address_space(3))) float *)(my_dist + d + a.reach), dz[r], 0, 0,
+                                        false);
+          }
+        }
+      }
+    }
+    if constexpr (FEAT & kCap) {
+#pragma unroll
+      for (int r = 0; r < 16; r++) dz[r] *= by_cap[r];
+    }
+    // dS is rounded to the rows' type, as K is; scale comes after the sum
+#pragma unroll
+    for (int v = 0; v < 2; v++) {
+      const Frag f = pack8<Frag>(dz + 8 * v);
+#pragma unroll
+      for (int d = 0; d < ND; d++) acc[d] = mfma16(KV::cols(kl, 16 * v, d, lane), f, acc[d]);
+    }
+  }
+
+  if (mine) {
+    T *o = (T *)x.g.dq.p + row * x.g.dq.row + head * x.g.dq.head;
+#pragma unroll
+    for (int d = 0; d < ND; d++)
+#pragma unroll
+      for (int g = 0; g < 4; g++) {
+        const int c = 32 * d + 8 * g + 4 * h;
+        if (c < a.dim)
+          store4(o + c, f4{acc[d][4 * g] * a.scale, acc[d][4 * g + 1] * a.scale, acc[d][4 * g + 2] * a.scale,
+                           acc[d][4 * g + 3] * a.scale});
+      }
+  }
+  if constexpr (FEAT & kBias) {
+    if (grad_table) {
+      // the ends: every lane's sums, in a fixed order of the lanes
+#pragma unroll
+      for (int o = 1; o < 64; o <<= 1) {
+        above += __shfl_xor(above, o);
+        below += __shfl_xor(below, o);
+      }
+      if (lane == 0) {
+        float *const d = dist + 2 * wave * span;
+        d[0] = below;
+        d[span - 1] = above;
+      }
+      __syncthreads();
+      for (int i = tid; i < span; i += THREADS) {
+        float v = 0.0f;
+#pragma unroll
+        for (int w = 0; w < 2 * Sh::WAVES; w++) v += dist[w * span + i];
+        dist_out[i] = v;
+      }
+    }
+  }
+}
+
+// ---- dK, dV -----------------------------------------------------------------
+
+template <class T, int DT>
+struct DkvShape {
+  static constexpr int WAVES = 4, THREADS = 256, KEYS = 128;
+  static constexpr int BQ = 32;
+  typedef Tile<T, DT, BQ, THREADS> QO;
+  // Q and dO twice, then lse, delta and the documents of the rows twice
+  static constexpr int STAT = 4 * QO::BYTES, DOCS = STAT + 4 * 4 * BQ, BIAS = DOCS + 2 * 4 * BQ;
+};
+
+template <class T, int DT, int FEAT>
+__global__ __launch_bounds__(256, sizeof(T) == 4 || DT == 128 ? 1 : 2) void attend_dkv_kernel(AttendArgs x) {
+  typedef DkvShape<T, DT> Sh;
+  typedef typename Sh::QO QO;
+  typedef typename Kind<T>::frag Frag;
+  constexpr int THREADS = Sh::THREADS, KEYS = Sh::KEYS, BQ = Sh::BQ, KS = DT / 16, ND = DT / 32;
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  const ixh_attend_args &a = x.a;
+  const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  float *const stat = (float *)(smem + Sh::STAT);
+  int *const qdocs = (int *)(smem + Sh::DOCS);
+  float *const bias = (float *)(smem + Sh::BIAS);
+
+  const int kvh = blockIdx.x % a.kv_heads;
+  int b;
+  int64_t blk;
+  find_block(a.k_offs, a.B, a.nk, KEYS, 1, blockIdx.x / a.kv_heads, &b, &blk);
+  const Seq s(a, b);
+  if (blk * KEYS >= s.nk) return;
+  const int first = (int)(blk * KEYS);
+  const int key = min(first + wave * 32 + (lane & 31), s.nk - 1);
+  const bool mine = first + wave * 32 + (lane & 31) < s.nk;
+  int lo, hi;  // places of the queries that see the key
+  query_bounds(a, s, key, &lo, &hi);
+  const int k_lo = __builtin_amdgcn_readlane(key, 0), k_hi = __builtin_amdgcn_readlane(key, 31);
+  const int lo_min = __builtin_amdgcn_readlane(lo, 0), lo_max = __builtin_amdgcn_readlane(lo, 31);
+  const int hi_min = __builtin_amdgcn_readlane(hi, 0), hi_max = __builtin_amdgcn_readlane(hi, 31);
+  if (hi < lo) lo = 1 << 30, hi = 1 << 30;
+  const unsigned width = hi - lo;
+  int t_begin, t_end;  // steps of BQ queries
+  {
+    int l, u, unused;
+    query_bounds(a, s, first, &l, &unused);
+    query_bounds(a, s, min(first + KEYS, s.nk) - 1, &unused, &u);
+    l -= s.shift, u -= s.shift;
+    t_begin = max(l, 0) / BQ;
+    t_end = u >= max(l, 0) ? min(u, s.nq - 1) / BQ + 1 : t_begin;
+    if (t_end < t_begin) t_end = t_begin;
+  }
+  const int64_t row = s.k0 + key;
+  const int kd = a.k_docs ? a.k_docs[row] : 0;
+  const int doc = kd < 0 ? -2 : kd;
+  const bool alive = !a.k_docs || kd >= 0;
+
+  Frag k[KS], v[KS];
+  {
+    const T *kr = (const T *)a.k.p + row * a.k.row + kvh * a.k.head;
+    const T *vr = (const T *)a.v.p + row * a.v.row + kvh * a.v.head;
+#pragma unroll
+    for (int i = 0; i < KS; i++) {
+      const bool in = 16 * i + 8 * h < a.dim && alive;
+      k[i] = load8(kr + 16 * i + 8 * h, in);
+      v[i] = load8(vr + 16 * i + 8 * h, in);
+    }
+  }
+  const Score sc(a, FEAT & kCap);
+  v16f dk[ND], dv[ND];
+#pragma unroll
+  for (int d = 0; d < ND; d++) dk[d] = v16f{}, dv[d] = v16f{};
+
+  QO qt, gt;
+  float lse = 0.0f, delta = 0.0f;
+  int qdoc = 0, buf = 0;
+  for (int g = 0; g < x.group; g++) {
+    const int head = kvh * x.group + g;
+    const T *const qb = (const T *)a.q.p + s.q0 * a.q.row + head * a.q.head;
+    const T *const gb = (const T *)x.g.d_out.p + s.q0 * x.g.d_out.row + head * x.g.d_out.head;
+    const float *const lse_of = a.lse + (int64_t)head * a.nq + s.q0;
+    const float *const delta_of = x.delta + (int64_t)head * a.nq + s.q0;
+    const float slope = (FEAT & kBias) && a.slopes ? -a.slopes[head] * kLog2e : 0.0f;
+    if constexpr (FEAT & kBias) {
+      if (a.table) {
+        __syncthreads();
+        load_bias<T>(a, head, bias, tid, THREADS);
+      }
+    }
+    auto fetch = [&](int t) {
+      qt.get(qb, a.q.row, t * BQ, s.nq, a.dim, tid);
+      gt.get(gb, x.g.d_out.row, t * BQ, s.nq, a.dim, tid);
+      if (tid < BQ) {
+        const int r = t * BQ + tid;
+        lse = r < s.nq ? lse_of[r] : -INFINITY;
+        delta = r < s.nq ? delta_of[r] : 0.0f;
+        if (a.q_docs) qdoc = r < s.nq ? max(a.q_docs[s.q0 + r], -1) : -1;
+      }
+    };
+    if (t_begin < t_end) fetch(t_begin);
+    for (int t = t_begin; t < t_end; t++, buf ^= 1) {
+      char *const ql = smem + buf * 2 * QO::BYTES, *const gl = ql + QO::BYTES;
+      float *const st = stat + buf * 2 * BQ;
+      {
+        // a row that sees nothing (lse -inf) is cleared: P is 0 at +inf
+        if (tid < BQ) {
+          st[tid] = lse > -INFINITY ? lse * kLog2e : INFINITY;
+          st[BQ + tid] = lse > -INFINITY ? delta : 0.0f;
+          qdocs[buf * BQ + tid] = qdoc;
+        }
+        __syncthreads();
+        auto keep = [&](int r) { return st[r] < INFINITY; };
+        qt.put(ql, a.dim, tid, false, keep);
+        gt.put(gl, a.dim, tid, false, keep);
+      }
+      __syncthreads();
+      if (t + 1 < t_end) fetch(t + 1);
+      const int p0 = t * BQ + s.shift;  // place of the step's first query
+      if (p0 > hi_max || p0 + BQ <= lo_min) continue;
+
+      v16f z = v16f{}, dp = v16f{};
+#pragma unroll
+      for (int i = 0; i < KS; i++) {
+        z = mfma16(QO::rows(ql, 0, i, lane), k[i], z);
+        dp = mfma16(QO::rows(gl, 0, i, lane), v[i], dp);
+      }
+      float by_cap[16];
+      shape_scores<T, FEAT>(z, by_cap, sc);
+      if constexpr (FEAT & kBias) {
+        const int d0 = key - p0 - 4 * h;  // distance at register 0, one less a row
+        if (a.slopes) {
+          const float f = (float)d0;
+#pragma unroll
+          for (int r = 0; r < 16; r++)
+            z[r] = __builtin_fmaf(slope, __builtin_fabsf(f - (float)(8 * (r >> 2) + (r & 3))), z[r]);
+        }
+        if (a.table) {
+          const int near = k_lo - p0 - 31, far = k_hi - p0;
+          if (near >= a.reach || far <= -a.reach) {
+            const float c = bias[near >= a.reach ? 2 * (a.reach + kBiasPad) : 0];
+#pragma unroll
+            for (int r = 0; r < 16; r++) z[r] += c;
+          } else {
+            const float *at = bias + d0 + a.reach + kBiasPad;
+#pragma unroll
+            for (int r = 0; r < 16; r++) z[r] += at[-(8 * (r >> 2) + (r & 3))];
+          }
+        }
+      }
+      float pr[16];
+#pragma unroll
+      for (int g4 = 0; g4 < 4; g4++) {
+        const f4 l = *(const f4 *)(st + 8 * g4 + 4 * h);
+#pragma unroll
+        for (int e = 0; e < 4; e++) pr[4 * g4 + e] = exp2_fast(z[4 * g4 + e] - l[e]);
+      }
+      if (a.q_docs || p0 < lo_max || p0 + BQ - 1 > hi_min) {
+        const unsigned e0 = p0 + 4 * h - lo;
+#pragma unroll
+        for (int r = 0; r < 16; r++)
+          if (e0 + (unsigned)(8 * (r >> 2) + (r & 3)) > width) pr[r] = 0.0f;
+        if (a.q_docs) {
+#pragma unroll
+          for (int g4 = 0; g4 < 4; g4++) {
+            const i4 d = *(const i4 *)(qdocs + buf * BQ + 8 * g4 + 4 * h);
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+              if (d[e] != doc) pr[4 * g4 + e] = 0.0f;
+          }
+        }
+      }
+      float ds[16];
+#pragma unroll
+      for (int g4 = 0; g4 < 4; g4++) {
+        const f4 dl = *(const f4 *)(st + BQ + 8 * g4 + 4 * h);
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          const int r = 4 * g4 + e;
+          ds[r] = pr[r] * (dp[r] - dl[e]);
+          if constexpr (FEAT & kCap) ds[r] *= by_cap[r];
+        }
+      }
+      // P and dS are rounded to the rows' type, as dO and Q are
+#pragma unroll
+      for (int w = 0; w < 2; w++) {
+        const Frag pf = pack8<Frag>(pr + 8 * w), sf = pack8<Frag>(ds + 8 * w);
+#pragma unroll
+        for (int d = 0; d < ND; d++) {
+          dv[d] = mfma16(QO::cols(gl, 16 * w, d, lane), pf, dv[d]);
+          dk[d] = mfma16(QO::cols(ql, 16 * w, d, lane), sf, dk[d]);
+        }
+      }
+    }
+  }
+  if (!mine) return;
+  T *ok = (T *)x.g.dk.p + row * x.g.dk.row + kvh * x.g.dk.head;
+  T *ov = (T *)x.g.dv.p + row * x.g.dv.row + kvh * x.g.dv.head;
+#pragma unroll
+  for (int d = 0; d < ND; d++)
+#pragma unroll
+    for (int g = 0; g < 4; g++) {
+      const int c = 32 * d + 8 * g + 4 * h;
+      if (c < a.dim) {
+        store4(ok + c, f4{dk[d][4 * g] * a.scale, dk[d][4 * g + 1] * a.scale, dk[d][4 * g + 2] * a.scale,
+                          dk[d][4 * g + 3] * a.scale});
+        store4(ov + c, f4{dv[d][4 * g], dv[d][4 * g + 1], dv[d][4 * g + 2], dv[d][4 * g + 3]});
+      }
+    }
+}
+
+// ---- the table's gradient ----------------------------------------------------
+
+// Sums of dZ by distance over the workgroups of attend_dq_kernel: a part of
+// them each block, four strands a distance.
+__global__ __launch_bounds__(256) void attend_dist_kernel(AttendArgs x) {
+  __shared__ float strand[4][64];
+  const int span = 2 * x.a.reach + 1, head = blockIdx.y, part = blockIdx.z;
+  const int i = blockIdx.x * 64 + (threadIdx.x & 63), w = threadIdx.x >> 6;
+  const int64_t per = (x.slots + x.dist_parts - 1) / x.dist_parts;
+  const int64_t end = min(x.slots, (part + 1) * per);
+  float v = 0.0f;
+  if (i < span)
+    for (int64_t slot = part * per + w; slot < end; slot += 4) v += x.dist[(slot * x.a.heads + head) * span + i];
+  strand[w][threadIdx.x & 63] = v;
+  __syncthreads();
+  if (w == 0 && i < span)
+    x.dist_sum[((int64_t)part * x.a.heads + head) * span + i] =
+        (strand[0][threadIdx.x] + strand[1][threadIdx.x]) + (strand[2][threadIdx.x] + strand[3][threadIdx.x]);
+}
+
+// The distances of each bucket: a block a head, the bucket's distances in
+// ascending order.
+template <class T>
+__global__ __launch_bounds__(256) void attend_dtable_kernel(AttendArgs x) {
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  const int span = 2 * x.a.reach + 1, head = blockIdx.x;
+  float *const sum = (float *)smem;
+  int *const of = (int *)(sum + span);
+  for (int i = threadIdx.x; i < span; i += 256) {
+    float v = 0.0f;
+    for (int part = 0; part < x.dist_parts; part++) v += x.dist_sum[((int64_t)part * x.a.heads + head) * span + i];
+    sum[i] = v;
+    of[i] = x.a.buckets[i];
+  }
+  __syncthreads();
+  for (int b = threadIdx.x; b < x.a.n_buckets; b += 256) {
+    float v = 0.0f;
+    for (int i = 0; i < span; i++) v += of[i] == b ? sum[i] : 0.0f;
+    ((T *)x.g.dtable)[(int64_t)b * x.a.heads + head] = (T)v;
+  }
+}
+
+template <class T, int DT, int FEAT>
+bool run_dq(const AttendArgs &x, hipStream_t s) {
+  typedef DqShape<T, DT> Sh;
+  const int len = (FEAT & kBias) && x.a.table ? attend_bias_len(x.a.reach) : 0;
+  const int shm = Sh::BIAS + 4 * len + (len ? 8 * 4 * (2 * x.a.reach + 1) : 0);
+  static PerDevice lds;
+  if (!lds_granted(lds, (const void *)attend_dq_kernel<T, DT, FEAT>, 160 << 10)) return false;
+  attend_dq_kernel<T, DT, FEAT><<<dim3((unsigned)(x.slots * x.a.heads)), Sh::THREADS, shm, s>>>(x);
+  return true;
+}
+template <class T, int DT, int FEAT>
+bool run_dkv(const AttendArgs &x, hipStream_t s) {
+  typedef DkvShape<T, DT> Sh;
+  const int shm = Sh::BIAS + ((FEAT & kBias) && x.a.table ? 4 * attend_bias_len(x.a.reach) : 0);
+  static PerDevice lds;
+  if (!lds_granted(lds, (const void *)attend_dkv_kernel<T, DT, FEAT>, 160 << 10)) return false;
+  attend_dkv_kernel<T, DT, FEAT><<<dim3((unsigned)(x.slots * x.a.kv_heads)), Sh::THREADS, shm, s>>>(x);
+  return true;
+}
+
+template <class T, int DT>
+bool by_feat(const AttendArgs &x, bool dq, hipStream_t s) {
+  const bool cap = x.a.cap > 0, bias = x.a.slopes || x.a.table;
+  if (dq) {
+    if (cap) return bias ? run_dq<T, DT, 3>(x, s) : run_dq<T, DT, 1>(x, s);
+    return bias ? run_dq<T, DT, 2>(x, s) : run_dq<T, DT, 0>(x, s);
+  }
+  if (cap) return bias ? run_dkv<T, DT, 3>(x, s) : run_dkv<T, DT, 1>(x, s);
+  return bias ? run_dkv<T, DT, 2>(x, s) : run_dkv<T, DT, 0>(x, s);
+}
+bool by_type(const AttendArgs &x, bool dq, hipStream_t s) {
+  const bool small = x.a.dim <= 64;
+  switch (x.a.type) {
+    case IXH_TYPE_F32: return small ? by_feat<float, 64>(x, dq, s) : by_feat<float, 128>(x, dq, s);
+    case IXH_TYPE_BF16: return small ? by_feat<__bf16, 64>(x, dq, s) : by_feat<__bf16, 128>(x, dq, s);
+    default: return small ? by_feat<_Float16, 64>(x, dq, s) : by_feat<_Float16, 128>(x, dq, s);
+  }
+}
+
+}  // namespace
+
+bool launch_attend_dq(const AttendArgs &x, hipStream_t s) { return by_type(x, true, s); }
+bool launch_attend_dkv(const AttendArgs &x, hipStream_t s) { return by_type(x, false, s); }
+
+void launch_attend_dtable(const AttendArgs &x, hipStream_t s) {
+  const int span = 2 * x.a.reach + 1;
+  attend_dist_kernel<<<dim3((span + 63) / 64, x.a.heads, x.dist_parts), 256, 0, s>>>(x);
+  const int shm = 8 * span;
+  switch (x.a.type) {
+    case IXH_TYPE_F32: attend_dtable_kernel<float><<<x.a.heads, 256, shm, s>>>(x); break;
+    case IXH_TYPE_BF16: attend_dtable_kernel<__bf16><<<x.a.heads, 256, shm, s>>>(x); break;
+    default: attend_dtable_kernel<_Float16><<<x.a.heads, 256, shm, s>>>(x); break;
+  }
+}
+
+}  // namespace ixh

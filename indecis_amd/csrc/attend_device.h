@@ -1,0 +1,326 @@
+// attend_device.h — what the float attention kernels share: fragments of
+// the three types, tiles of rows in LDS, the masks' bounds, the scores.
+//
+// Layout. Every product is taken with a 32x32x16 MFMA (for float32 eight
+// 32x32x2 ones over the same fragments): lane l supplies row l % 32 of A
+// and column l % 32 of B, eight values each of the 16 of k; which eight is
+// free as long as A and B agree. The result's lane l holds column l % 32,
+// rows 8 (r / 4) + 4 (l / 32) + r % 4, r = 0..15. So a product whose columns
+// are queries leaves in a lane 4 keys of every 8 of one query: taken in that
+// order they are the next product's B fragment over k = keys as they stand,
+// and its A fragment is read from LDS transposed in the same order
+// (ds_read_b64_tr_b16: 4 rows of 16 columns a 16-lane group). No score
+// leaves the registers, and a query's softmax is its lane's own.
+#pragma once
+#include <hip/hip_bf16.h>
+#include <hip/hip_fp16.h>
+
+#include "attend.h"
+
+namespace ixh {
+
+typedef float v16f __attribute__((ext_vector_type(16)));
+typedef float f4 __attribute__((ext_vector_type(4)));
+typedef short v4s __attribute__((ext_vector_type(4)));
+typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
+typedef _Float16 v8h __attribute__((ext_vector_type(8)));
+struct alignas(16) v8f {
+  f4 lo, hi;
+};
+typedef int i4 __attribute__((ext_vector_type(4)));
+
+constexpr float kLog2e = 1.44269504088896340736f;
+constexpr float kLn2 = 0.69314718055994530942f;
+
+template <class T>
+struct Kind;
+template <>
+struct Kind<__bf16> {
+  typedef v8bf frag;
+};
+template <>
+struct Kind<_Float16> {
+  typedef v8h frag;
+};
+template <>
+struct Kind<float> {
+  typedef v8f frag;
+};
+
+__device__ __forceinline__ v16f mfma16(v8bf a, v8bf b, v16f c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ v16f mfma16(v8h a, v8h b, v16f c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+// Value e of both halves of the wave together are one 32x32x2 product.
+__device__ __forceinline__ v16f mfma16(const v8f &a, const v8f &b, v16f c) {
+#pragma unroll
+  for (int e = 0; e < 4; e++) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a.lo[e], b.lo[e], c, 0, 0, 0);
+#pragma unroll
+  for (int e = 0; e < 4; e++) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a.hi[e], b.hi[e], c, 0, 0, 0);
+  return c;
+}
+
+template <class F>
+__device__ __forceinline__ float frag_at(const F &f, int e) {
+  return (float)f[e];
+}
+__device__ __forceinline__ float frag_at(const v8f &f, int e) { return e < 4 ? f.lo[e] : f.hi[e - 4]; }
+
+// Eight accumulator values as a fragment of the type, rounded to nearest even.
+template <class F>
+__device__ __forceinline__ F pack8(const float *p) {
+  F f;
+#pragma unroll
+  for (int e = 0; e < 8; e++) f[e] = p[e];
+  return f;
+}
+template <>
+__device__ __forceinline__ v8f pack8<v8f>(const float *p) {
+  v8f f;
+#pragma unroll
+  for (int e = 0; e < 4; e++) f.lo[e] = p[e], f.hi[e] = p[e + 4];
+  return f;
+}
+template <>
+__device__ __forceinline__ v8bf pack8<v8bf>(const float *p) {
+  v8bf f;
+#pragma unroll
+  for (int e = 0; e < 8; e++) f[e] = (__bf16)p[e];
+  return f;
+}
+template <>
+__device__ __forceinline__ v8h pack8<v8h>(const float *p) {
+  v8h f;
+#pragma unroll
+  for (int e = 0; e < 8; e++) f[e] = (_Float16)p[e];
+  return f;
+}
+
+// Eight values at p; none past `valid` (0 or 8) are read.
+template <class T>
+__device__ __forceinline__ typename Kind<T>::frag load8(const T *p, bool valid) {
+  typename Kind<T>::frag f{};
+  if (valid) f = *(const typename Kind<T>::frag *)p;
+  return f;
+}
+
+// Four consecutive values, rounded once.
+__device__ __forceinline__ void store4(float *p, f4 v) { *(f4 *)p = v; }
+__device__ __forceinline__ void store4(__bf16 *p, f4 v) {
+  typedef __bf16 b4 __attribute__((ext_vector_type(4)));
+  b4 o = {(__bf16)v[0], (__bf16)v[1], (__bf16)v[2], (__bf16)v[3]};
+  *(b4 *)p = o;
+}
+__device__ __forceinline__ void store4(_Float16 *p, f4 v) {
+  typedef _Float16 h4 __attribute__((ext_vector_type(4)));
+  h4 o = {(_Float16)v[0], (_Float16)v[1], (_Float16)v[2], (_Float16)v[3]};
+  *(h4 *)p = o;
+}
+
+__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// The other half of the wave's value at the same column.
+__device__ __forceinline__ float other_half(float v) {
+  typedef unsigned u2 __attribute__((ext_vector_type(2)));
+  const unsigned u = __builtin_bit_cast(unsigned, v);
+  const u2 r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  return __builtin_bit_cast(float, (__lane_id() & 32) ? r[0] : r[1]);
+}
+// A fixed order of the two halves, so that both get the same bits.
+__device__ __forceinline__ float half_sum(float v) { return v + other_half(v); }
+__device__ __forceinline__ float half_max(float v) { return __builtin_fmaxf(v, other_half(v)); }
+
+// ---- tiles of rows in LDS ---------------------------------------------------
+// R rows of DT values, 16-byte pieces; piece c of row r stands at c ^ (r & 7),
+// so that the 16 rows a quarter-wave reads of one column of pieces, and the 8
+// rows a transposed read touches, lie in different banks.
+template <class T, int DT, int R, int THREADS>
+struct Tile {
+  static constexpr int EPC = 16 / (int)sizeof(T);  // values a piece
+  static constexpr int CH = DT / EPC;              // pieces a row
+  static constexpr int RB = DT * (int)sizeof(T);   // bytes a row
+  static constexpr int BYTES = R * RB;
+  static constexpr int N = R * CH / THREADS;       // pieces a thread
+  static_assert(N * THREADS == R * CH && CH >= 8, "");
+  i4 part[N];
+
+  // Starts the loads of rows r0.. of the sequence (n rows in all, from base):
+  // a row past the last and a piece past `dim` are read where there is one
+  // and dropped in put().
+  __device__ __forceinline__ void get(const T *base, int64_t stride, int r0, int n, int dim, int tid) {
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+      const int at = tid + i * THREADS, r = at / CH, c = at % CH;
+      const int row = min(r0 + r, n - 1);
+      const int col = c * EPC < dim ? c * EPC : 0;
+      part[i] = *(const i4 *)(base + row * stride + col);
+    }
+  }
+  // Writes them. keep(r): whether row r of the tile is used; others are 0.
+  template <class Keep>
+  __device__ __forceinline__ void put(char *lds, int dim, int tid, bool all, Keep keep) {
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+      const int at = tid + i * THREADS, r = at / CH, c = at % CH;
+      i4 v = part[i];
+      if (!all && !(c * EPC < dim && keep(r))) v = i4{0, 0, 0, 0};
+      *(i4 *)(lds + r * RB + ((c ^ (r & 7)) << 4)) = v;
+    }
+  }
+
+  // A's fragment of rows row0 + l % 32 at k step s (16 values of a row).
+  __device__ static __forceinline__ typename Kind<T>::frag rows(const char *lds, int row0, int s, int lane) {
+    const int r = row0 + (lane & 31), h = lane >> 5;
+    typename Kind<T>::frag f;
+    if constexpr (sizeof(T) == 2) {
+      f = *(const typename Kind<T>::frag *)(lds + r * RB + (((2 * s + h) ^ (r & 7)) << 4));
+    } else {
+      const int c = 4 * s + 2 * h;
+      f.lo = *(const f4 *)(lds + r * RB + ((c ^ (r & 7)) << 4));
+      f.hi = *(const f4 *)(lds + r * RB + (((c + 1) ^ (r & 7)) << 4));
+    }
+    return f;
+  }
+  // A's fragment of columns 32 dt + l % 32 over the 16 rows from row0, rows
+  // in the order in which a result's registers hold them.
+  __device__ static __forceinline__ typename Kind<T>::frag cols(const char *lds, int row0, int dt, int lane) {
+    const int h = lane >> 5;
+    typename Kind<T>::frag f;
+    if constexpr (sizeof(T) == 2) {
+      const int a = lane & 15, g = (lane >> 4) & 1;
+      const int r = row0 + 4 * h + (a >> 2), c = 4 * dt + 2 * g + ((a >> 1) & 1);
+      const char *p = lds + r * RB + ((c ^ (r & 7)) << 4) + ((a & 1) << 3);
+      typedef __attribute__((address_space(3))) v4s lv4s;
+      union {
+        v4s q[2];
+        typename Kind<T>::frag f;
+      } u;
+      u.q[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lv4s *)p);
+      u.q[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lv4s *)(p + 8 * RB));
+      f = u.f;
+    } else {
+      const int d = 32 * dt + (lane & 31), c = d >> 2;
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        const int r = row0 + 4 * h + j;
+        const char *p = lds + r * RB + ((c ^ (r & 7)) << 4) + ((d & 3) << 2);
+        f.lo[j] = *(const float *)p;
+        f.hi[j] = *(const float *)(p + 8 * RB);
+      }
+    }
+    return f;
+  }
+};
+
+// ---- sequences and masks ----------------------------------------------------
+
+// offs[i] as a row of an array of n rows, whatever it holds.
+__device__ __forceinline__ int row_at(const int32_t *offs, int i, int n) { return min(max(offs[i], 0), n); }
+
+// The sequence of a slot (attend_slots) and its block of rows: a search by
+// the whole wave, 64 sequences a step.
+__device__ __forceinline__ void find_block(const int32_t *offs, int B, int n, int rows, int pack, int64_t slot, int *seq,
+                                           int64_t *block) {
+  const int lane = __lane_id();
+  int lo = 0, count = B;
+  while (count > 1) {
+    const int step = (count + 63) / 64;
+    const int b = lo + lane * step;
+    const bool mine = lane * step < count && (int64_t)row_at(offs, b, n) * pack / rows + b <= slot;
+    const int at = max(0, __popcll(__ballot(mine)) - 1);
+    lo += at * step;
+    count = min(step, count - at * step);
+  }
+  lo = __builtin_amdgcn_readfirstlane(lo);
+  *seq = lo;
+  *block = slot - ((int64_t)row_at(offs, lo, n) * pack / rows + lo);
+}
+
+// One sequence: its rows in the packed arrays.
+struct Seq {
+  int q0, nq, k0, nk, shift, prefix;  // shift: a query's place among the keys less its row
+  __device__ __forceinline__ Seq(const ixh_attend_args &a, int b) {
+    q0 = row_at(a.q_offs, b, a.nq);
+    nq = max(row_at(a.q_offs, b + 1, a.nq) - q0, 0);
+    k0 = row_at(a.k_offs, b, a.nk);
+    nk = max(row_at(a.k_offs, b + 1, a.nk) - k0, 0);
+    shift = nk - nq;
+    prefix = a.prefix ? a.prefix[b] : 0;
+  }
+};
+
+// The keys lo..hi that the query at place p sees (documents apart); empty
+// where hi < lo. Both ends grow with p.
+__device__ __forceinline__ void key_bounds(const ixh_attend_args &a, const Seq &s, int p, int *lo, int *hi) {
+  int h = s.nk - 1, l = 0;
+  if (a.causal) h = min(h, max(p, s.prefix - 1));
+  if (a.window >= 0) {
+    h = min((int64_t)h, (int64_t)p + a.window);
+    l = max((int64_t)l, (int64_t)p - a.window);
+  }
+  *lo = l;
+  *hi = h;
+}
+// The places lo..hi of the queries that see key j.
+__device__ __forceinline__ void query_bounds(const ixh_attend_args &a, const Seq &s, int j, int *lo, int *hi) {
+  int l = s.shift, h = s.nk - 1;
+  if (a.causal && j >= s.prefix) l = max(l, j);
+  if (a.window >= 0) {
+    l = max((int64_t)l, (int64_t)j - a.window);
+    h = min((int64_t)h, (int64_t)j + a.window);
+  }
+  *lo = l;
+  *hi = h;
+}
+
+// ---- scores -----------------------------------------------------------------
+// FEAT: 1 a tanh cap, 2 a bias by distance.
+enum { kCap = 1, kBias = 2 };
+
+// Constants of a call's scores in base 2: z = c1 * s, or, capped,
+// z = c2 tanh(s * scale / cap); the softmax is 2^(z - maximum).
+struct Score {
+  float c1, c2;
+  __device__ __forceinline__ explicit Score(const ixh_attend_args &a, bool cap) {
+    if (cap) {
+      c1 = a.scale / a.cap;
+      c2 = a.cap * kLog2e;
+    } else {
+      c1 = a.scale * kLog2e;
+      c2 = 0;
+    }
+  }
+};
+
+// tanh(x) = 1 - 2u, u = 1 / (1 + e^2x), with the hardware's exponential and
+// reciprocal: off by about 1e-7 of 1, which next to a 16-bit result is
+// nothing; float32 takes the library's tanh. *u serves the derivative,
+// 1 - tanh^2 = 4 u (1 - u).
+template <class T>
+__device__ __forceinline__ float tanh_of(float x, float *u) {
+  if constexpr (sizeof(T) == 4) {
+    const float t = tanhf(x);
+    *u = 0.5f - 0.5f * t;
+    return t;
+  } else {
+    const float e = exp2_fast(x * (2 * kLog2e));
+    *u = __builtin_amdgcn_rcpf(1.0f + e);
+    return __builtin_fmaf(-2.0f, *u, 1.0f);
+  }
+}
+
+// The bias of one head: slope (base 2) and the table by distance, copied to
+// LDS in base 2 with its ends drawn out by kBiasPad.
+template <class T>
+__device__ __forceinline__ void load_bias(const ixh_attend_args &a, int head, float *lds, int tid, int threads) {
+  const int len = attend_bias_len(a.reach);
+  for (int i = tid; i < len; i += threads) {
+    const int d = min(max(i - a.reach - kBiasPad, -a.reach), a.reach);
+    const int b = a.buckets[d + a.reach];
+    lds[i] = b >= 0 && b < a.n_buckets ? (float)((const T *)a.table)[(int64_t)b * a.heads + head] * kLog2e : 0.0f;
+  }
+}
+
+}  // namespace ixh

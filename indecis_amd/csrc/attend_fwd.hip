@@ -1,0 +1,399 @@
+// attend_fwd.hip — attention of float rows with shaped scores: one pass over
+// the keys with a running maximum and sum a query.
+//
+// A workgroup of 4 waves has 128 query rows of a sequence and head, 32 a
+// wave (one wave and 32 rows where sequences are short). K and V come through
+// LDS, 64 keys a step in two buffers, loaded into registers a step ahead.
+// The scores are taken transposed (keys x queries, attend_device.h): a lane
+// has one query, so maximum, sum and rescaling are its own, and the
+// probabilities go into the second product from the registers they are in.
+#include "attend_device.h"
+#include "ixh_internal.h"
+
+namespace ixh {
+namespace {
+
+constexpr int kDocWords = 64;  // 64 steps of keys a word; later steps are taken as live
+
+template <class T, int DT, int WAVES>
+struct FwdShape {
+  static constexpr int THREADS = 64 * WAVES, ROWS = 32 * WAVES;
+  static constexpr int BK = attend_keys(sizeof(T), WAVES == 1), NS = BK / 32;
+  typedef Tile<T, DT, BK, THREADS> KV;
+  // LDS: K and V twice, the key documents twice, the live and the pure steps
+  // of documents, then the bias
+  static constexpr int DOCS = 4 * KV::BYTES, LIVE = DOCS + 2 * 4 * BK, BIAS = LIVE + 16 * kDocWords;
+};
+
+template <class T, int DT, int WAVES, int FEAT>
+__global__ __launch_bounds__(64 * WAVES, 2) void attend_fwd_kernel(AttendArgs x) {
+  typedef FwdShape<T, DT, WAVES> Sh;
+  typedef typename Sh::KV KV;
+  typedef typename Kind<T>::frag Frag;
+  constexpr int THREADS = Sh::THREADS, ROWS = Sh::ROWS, BK = Sh::BK, NS = Sh::NS, KS = DT / 16, ND = DT / 32;
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  const ixh_attend_args &a = x.a;
+  const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  int *const kdocs = (int *)(smem + Sh::DOCS);
+  uint64_t *const live = (uint64_t *)(smem + Sh::LIVE), *const pure = live + kDocWords;
+  float *const bias = (float *)(smem + Sh::BIAS);
+
+  // last blocks first: under a causal mask they have the most keys
+  const int pack = x.pack, nh = pack > 1 ? a.kv_heads : a.heads;
+  const int hb = blockIdx.x % nh;
+  int b;
+  int64_t blk;
+  find_block(a.q_offs, a.B, a.nq, ROWS, pack, x.slots - 1 - blockIdx.x / nh, &b, &blk);
+  const Seq s(a, b);
+  const int64_t rows = (int64_t)s.nq * pack;
+  if (blk * ROWS >= rows) return;
+  const int kvh = pack > 1 ? hb : hb / x.group;
+
+  // the lane's query: row, head, place; rows past the last repeat it
+  const int64_t r = min(blk * ROWS + wave * 32 + (lane & 31), rows - 1);
+  const bool mine = blk * ROWS + wave * 32 + (lane & 31) < rows;
+  const int tok = pack > 1 ? (int)(r / pack) : (int)r, sub = pack > 1 ? (int)(r - (int64_t)tok * pack) : 0;
+  const int head = pack > 1 ? hb * pack + sub : hb;
+  const int p = tok + s.shift;
+  int lo, hi;
+  key_bounds(a, s, p, &lo, &hi);
+  const int p_lo = __builtin_amdgcn_readlane(p, 0), p_hi = __builtin_amdgcn_readlane(p, 31);
+  const int lo_min = __builtin_amdgcn_readlane(lo, 0), lo_max = __builtin_amdgcn_readlane(lo, 31);
+  const int hi_min = __builtin_amdgcn_readlane(hi, 0), hi_max = __builtin_amdgcn_readlane(hi, 31);
+  if (hi < lo) lo = 1 << 30, hi = 1 << 30;  // sees nothing: no key is there
+  const unsigned width = hi - lo;
+
+  // the workgroup's steps of keys
+  int t_begin, t_end;
+  {
+    int l, u, unused;
+    const int64_t last = min(blk * ROWS + ROWS, rows) - 1;
+    key_bounds(a, s, (int)(blk * ROWS / pack) + s.shift, &l, &unused);
+    key_bounds(a, s, (int)(last / pack) + s.shift, &unused, &u);
+    t_begin = l / BK;
+    t_end = u >= l ? u / BK + 1 : t_begin;
+    if (x.splits > 1) {
+      const int per = (t_end - t_begin + x.splits - 1) / x.splits;
+      t_begin = min(t_begin + per * (int)blockIdx.y, t_end);
+      t_end = min(t_begin + per, t_end);
+    }
+  }
+
+  // documents: which steps hold a key of one of this block's, and which hold
+  // one document only, this block's
+  int doc = 0;
+  if (a.q_docs) {
+    doc = max(a.q_docs[s.q0 + tok], -1);
+    // over the workgroup's rows
+    const int first = (int)(blk * ROWS / pack), last = (int)((min(blk * ROWS + ROWS, rows) - 1) / pack);
+    int all_mn = INT32_MAX, all_mx = -1;
+    bool none = false;
+    for (int i = first + (lane & 31); i <= last; i += 32) {
+      const int d = a.q_docs[s.q0 + i];
+      none |= d < 0;
+      all_mn = min(all_mn, d < 0 ? INT32_MAX : d);
+      all_mx = max(all_mx, d);
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) {
+      all_mn = min(all_mn, __shfl_xor(all_mn, o));
+      all_mx = max(all_mx, __shfl_xor(all_mx, o));
+    }
+    const bool one = all_mn == all_mx && !__ballot(none);
+    for (int w = wave; w < kDocWords && t_begin + 64 * w < t_end; w += WAVES) {
+      const int t = t_begin + 64 * w + lane;
+      int kmn = INT32_MAX, kmx = -1;
+      bool bad = t >= t_end || t * BK + BK > s.nk;
+      if (t < t_end) {
+        const int32_t *kd = a.k_docs + s.k0;
+#pragma unroll 32
+        for (int i = 0; i < BK; i++) {
+          const int d = kd[min(t * BK + i, s.nk - 1)];
+          bad |= d < 0;
+          kmn = min(kmn, d < 0 ? INT32_MAX : d);
+          kmx = max(kmx, d);
+        }
+      }
+      const bool some = kmx >= 0 && all_mx >= 0 && kmn <= all_mx && kmx >= all_mn;
+      const uint64_t lv = __ballot(some), pr = __ballot(some && one && !bad && kmn == kmx && kmn == all_mn);
+      if (lane == 0) live[w] = lv, pure[w] = pr;
+    }
+  }
+  if constexpr (FEAT & kBias) {
+    if (a.table)
+      for (int i = 0; i < pack; i++)
+        load_bias<T>(a, pack > 1 ? hb * pack + i : hb, bias + i * attend_bias_len(a.reach), tid, THREADS);
+  }
+  if (a.q_docs || (FEAT & kBias)) __syncthreads();
+
+  auto next = [&](int t) {
+    if (!a.q_docs) return t;
+    while (t < t_end) {
+      const int i = t - t_begin;
+      if (i >= 64 * kDocWords) return t;
+      const uint64_t w = live[i >> 6] >> (i & 63);
+      const int skip = w ? __builtin_ctzll(w) : 64 - (i & 63);
+      const int n = __builtin_amdgcn_readfirstlane(skip);
+      t += n;
+      if (n == 0) return t;
+    }
+    return t_end;
+  };
+
+  // Q's fragments, columns past dim 0
+  Frag q[KS];
+  {
+    const T *qr = (const T *)a.q.p + (s.q0 + tok) * a.q.row + head * a.q.head;
+#pragma unroll
+    for (int i = 0; i < KS; i++) q[i] = load8(qr + 16 * i + 8 * h, 16 * i + 8 * h < a.dim);
+  }
+  const T *const kb = (const T *)a.k.p + s.k0 * a.k.row + kvh * a.k.head;
+  const T *const vb = (const T *)a.v.p + s.k0 * a.v.row + kvh * a.v.head;
+  const Score sc(a, FEAT & kCap);
+  const float slope = (FEAT & kBias) && a.slopes ? -a.slopes[head] * kLog2e : 0.0f;
+  const float *const tab = bias + sub * attend_bias_len(a.reach);
+
+  v16f acc[ND];
+#pragma unroll
+  for (int d = 0; d < ND; d++) acc[d] = v16f{};
+  float m = -INFINITY, ref = 0.0f, sum = 0.0f;  // maximum so far; what scores are taken against
+
+  KV kt, vt;
+  int kdoc = 0;
+  auto fetch = [&](int t) {
+    kt.get(kb, a.k.row, t * BK, s.nk, a.dim, tid);
+    vt.get(vb, a.v.row, t * BK, s.nk, a.dim, tid);
+    if (a.q_docs && tid < BK) kdoc = t * BK + tid < s.nk ? a.k_docs[s.k0 + t * BK + tid] : -1;
+  };
+
+  int buf = 0;
+  int t = next(t_begin);
+  if (t < t_end) fetch(t);
+  while (t < t_end) {
+    char *const kl = smem + buf * 2 * KV::BYTES, *const vl = kl + KV::BYTES;
+    const bool dead = a.q_docs && !(t - t_begin < 64 * kDocWords && (pure[(t - t_begin) >> 6] >> ((t - t_begin) & 63) & 1));
+    {
+      // keys that no query sees hold anything: their rows are cleared
+      const bool all = a.dim == DT && t * BK + BK <= s.nk && !dead;
+      if (dead) {
+        if (tid < BK) kdocs[buf * BK + tid] = kdoc < 0 ? -2 : kdoc;
+        __syncthreads();
+      }
+      auto keep = [&](int row) { return t * BK + row < s.nk && (!dead || kdocs[buf * BK + row] >= 0); };
+      kt.put(kl, a.dim, tid, all, keep);
+      vt.put(vl, a.dim, tid, all, keep);
+    }
+    __syncthreads();
+    const int tn = next(t + 1);
+    if (tn < t_end) fetch(tn);
+
+    const int j0 = t * BK;
+    if (j0 <= hi_max && j0 + BK > lo_min) {
+      v16f z[NS];
+#pragma unroll
+      for (int u = 0; u < NS; u++) {
+        z[u] = v16f{};
+#pragma unroll
+        for (int i = 0; i < KS; i++) z[u] = mfma16(KV::rows(kl, 32 * u, i, lane), q[i], z[u]);
+      }
+      const bool masked = dead || j0 < lo_max || j0 + BK - 1 > hi_min;
+      if constexpr (FEAT != 0) {
+#pragma unroll
+        for (int u = 0; u < NS; u++) {
+          const int d0 = j0 + 32 * u + 4 * h - p;  // distance of register 0
+          if constexpr (FEAT & kCap) {
+#pragma unroll
+            for (int r = 0; r < 16; r++) {
+              float unused;
+              z[u][r] = sc.c2 * tanh_of<T>(z[u][r] * sc.c1, &unused);
+            }
+          } else {
+#pragma unroll
+            for (int r = 0; r < 16; r++) z[u][r] *= sc.c1;
+          }
+          if constexpr (FEAT & kBias) {
+            if (a.slopes) {
+              const float f = (float)d0;
+#pragma unroll
+              for (int r = 0; r < 16; r++)
+                z[u][r] = __builtin_fmaf(slope, __builtin_fabsf(f + (float)(8 * (r >> 2) + (r & 3))), z[u][r]);
+            }
+            if (a.table) {
+              const int near = j0 + 32 * u - p_hi, far = j0 + 32 * u + 31 - p_lo;
+              if (near >= a.reach || far <= -a.reach) {
+                const float c = tab[near >= a.reach ? 2 * (a.reach + kBiasPad) : 0];
+#pragma unroll
+                for (int r = 0; r < 16; r++) z[u][r] += c;
+              } else {
+                const float *at = tab + d0 + a.reach + kBiasPad;
+#pragma unroll
+                for (int r = 0; r < 16; r++) z[u][r] += at[8 * (r >> 2) + (r & 3)];
+              }
+            }
+          }
+        }
+      }
+      if (masked) {
+#pragma unroll
+        for (int u = 0; u < NS; u++) {
+          const unsigned e0 = j0 + 32 * u + 4 * h - lo;
+#pragma unroll
+          for (int r = 0; r < 16; r++)
+            if (e0 + (unsigned)(8 * (r >> 2) + (r & 3)) > width) z[u][r] = -INFINITY;
+          if (dead) {
+#pragma unroll
+            for (int g = 0; g < 4; g++) {
+              const i4 d = *(const i4 *)(kdocs + buf * BK + 32 * u + 8 * g + 4 * h);
+#pragma unroll
+              for (int e = 0; e < 4; e++)
+                if (d[e] != doc) z[u][4 * g + e] = -INFINITY;
+            }
+          }
+        }
+      }
+      float top = z[0][0];
+#pragma unroll
+      for (int u = 0; u < NS; u++)
+#pragma unroll
+        for (int r = 0; r < 16; r++) top = __builtin_fmaxf(top, z[u][r]);
+      top = half_max(top);
+      if constexpr (FEAT == 0) top *= sc.c1;
+      // the sums keep an old maximum until it is 2^8 short: they stay far
+      // inside every type's range, and few steps rescale
+      if (__ballot(top > m + 8.0f)) {
+        const float next_m = __builtin_fmaxf(m, top);
+        const float f = m == -INFINITY ? 0.0f : exp2_fast(m - next_m);
+        m = next_m;
+        ref = m == -INFINITY ? 0.0f : m;
+        sum *= f;
+#pragma unroll
+        for (int d = 0; d < ND; d++)
+#pragma unroll
+          for (int r = 0; r < 16; r++) acc[d][r] *= f;
+      }
+#pragma unroll
+      for (int u = 0; u < NS; u++) {
+        float part = 0.0f, pr[16];
+#pragma unroll
+        for (int r = 0; r < 16; r++) {
+          pr[r] = exp2_fast(FEAT == 0 ? __builtin_fmaf(z[u][r], sc.c1, -ref) : z[u][r] - ref);
+          part += pr[r];
+        }
+        sum += part;
+        // the probabilities are rounded to the rows' type here, as V is: the
+        // product's sum stays in 32 bits
+#pragma unroll
+        for (int v = 0; v < 2; v++) {
+          const Frag pf = pack8<Frag>(pr + 8 * v);
+#pragma unroll
+          for (int d = 0; d < ND; d++) acc[d] = mfma16(KV::cols(vl, 32 * u + 16 * v, d, lane), pf, acc[d]);
+        }
+      }
+    }
+    buf ^= 1;
+    t = tn;
+  }
+
+  sum = half_sum(sum);
+  if (!mine) return;
+  const int64_t row = s.q0 + tok;
+  if (x.splits > 1) {
+    const int64_t at = ((int64_t)blockIdx.y * a.nq + row) * a.heads + head;
+    float *o = x.part_o + at * a.dim;
+#pragma unroll
+    for (int d = 0; d < ND; d++)
+#pragma unroll
+      for (int g = 0; g < 4; g++) {
+        const int c = 32 * d + 8 * g + 4 * h;
+        if (c < a.dim) *(f4 *)(o + c) = f4{acc[d][4 * g], acc[d][4 * g + 1], acc[d][4 * g + 2], acc[d][4 * g + 3]};
+      }
+    if (h == 0) x.part_ml[2 * at] = m, x.part_ml[2 * at + 1] = sum;
+    return;
+  }
+  const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
+  T *o = (T *)a.o.p + row * a.o.row + head * a.o.head;
+#pragma unroll
+  for (int d = 0; d < ND; d++)
+#pragma unroll
+    for (int g = 0; g < 4; g++) {
+      const int c = 32 * d + 8 * g + 4 * h;
+      if (c < a.dim)
+        store4(o + c, f4{acc[d][4 * g] * inv, acc[d][4 * g + 1] * inv, acc[d][4 * g + 2] * inv, acc[d][4 * g + 3] * inv});
+    }
+  if (a.lse && h == 0) a.lse[(int64_t)head * a.nq + row] = (ref + __builtin_amdgcn_logf(sum)) * kLn2;
+}
+
+// The parts of the keys joined: a thread has four columns of a query's head.
+template <class T>
+__global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs x) {
+  const ixh_attend_args &a = x.a;
+  const int quads = a.dim / 4;
+  const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t rh = at / quads;
+  const int c = (int)(at - rh * quads) * 4;
+  const int64_t row = rh / a.heads;
+  const int head = (int)(rh - row * a.heads);
+  if (row >= row_at(a.q_offs, a.B, a.nq) || row < row_at(a.q_offs, 0, a.nq)) return;
+  float m = -INFINITY;
+  const int64_t step = (int64_t)a.nq * a.heads;
+  for (int i = 0; i < x.splits; i++) m = __builtin_fmaxf(m, x.part_ml[2 * (i * step + rh)]);
+  const float ref = m == -INFINITY ? 0.0f : m;
+  f4 o{};
+  float sum = 0.0f;
+  for (int i = 0; i < x.splits; i++) {
+    const float f = exp2_fast(x.part_ml[2 * (i * step + rh)] - ref);
+    sum = __builtin_fmaf(f, x.part_ml[2 * (i * step + rh) + 1], sum);
+    const f4 v = *(const f4 *)(x.part_o + (i * step + rh) * a.dim + c);
+#pragma unroll
+    for (int e = 0; e < 4; e++) o[e] = __builtin_fmaf(f, v[e], o[e]);
+  }
+  const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
+  store4((T *)a.o.p + row * a.o.row + head * a.o.head + c, o * inv);
+  if (a.lse && c == 0) a.lse[(int64_t)head * a.nq + row] = (ref + __builtin_amdgcn_logf(sum)) * kLn2;
+}
+
+template <class T, int DT, int WAVES, int FEAT>
+bool launch(const AttendArgs &x, hipStream_t s) {
+  typedef FwdShape<T, DT, WAVES> Sh;
+  const int shm = Sh::BIAS + ((FEAT & kBias) && x.a.table ? 4 * x.pack * attend_bias_len(x.a.reach) : 0);
+  static PerDevice lds;
+  if (!lds_granted(lds, (const void *)attend_fwd_kernel<T, DT, WAVES, FEAT>, 160 << 10)) return false;
+  const dim3 grid((unsigned)(x.slots * (x.pack > 1 ? x.a.kv_heads : x.a.heads)), x.splits);
+  attend_fwd_kernel<T, DT, WAVES, FEAT><<<grid, Sh::THREADS, shm, s>>>(x);
+  return true;
+}
+
+template <class T, int DT, int WAVES>
+bool by_feat(const AttendArgs &x, hipStream_t s) {
+  const bool cap = x.a.cap > 0, bias = x.a.slopes || x.a.table;
+  if (cap) return bias ? launch<T, DT, WAVES, 3>(x, s) : launch<T, DT, WAVES, 1>(x, s);
+  return bias ? launch<T, DT, WAVES, 2>(x, s) : launch<T, DT, WAVES, 0>(x, s);
+}
+template <class T>
+bool by_dim(const AttendArgs &x, bool few, hipStream_t s) {
+  if (x.a.dim <= 64) return few ? by_feat<T, 64, 1>(x, s) : by_feat<T, 64, 4>(x, s);
+  return few ? by_feat<T, 128, 1>(x, s) : by_feat<T, 128, 4>(x, s);
+}
+
+}  // namespace
+
+bool launch_attend_fwd(const AttendArgs &x, bool few, hipStream_t s) {
+  switch (x.a.type) {
+    case IXH_TYPE_F32: return by_dim<float>(x, few, s);
+    case IXH_TYPE_BF16: return by_dim<__bf16>(x, few, s);
+    default: return by_dim<_Float16>(x, few, s);
+  }
+}
+
+void launch_attend_join(const AttendArgs &x, hipStream_t s) {
+  const int64_t n = (int64_t)x.a.nq * x.a.heads * (x.a.dim / 4);
+  const unsigned grid = (unsigned)((n + 255) / 256);
+  switch (x.a.type) {
+    case IXH_TYPE_F32: attend_join_kernel<float><<<grid, 256, 0, s>>>(x); break;
+    case IXH_TYPE_BF16: attend_join_kernel<__bf16><<<grid, 256, 0, s>>>(x); break;
+    default: attend_join_kernel<_Float16><<<grid, 256, 0, s>>>(x); break;
+  }
+}
+
+}  // namespace ixh
