@@ -133,8 +133,9 @@ Plan plan_forward(AttendArgs &x) {
   const int64_t groups = x.slots * (x.pack > 1 ? a.kv_heads : a.heads);
   const int64_t steps = a.nk / B / attend_keys(type_size(a.type), p.few);
   x.splits = 1;
-  if (groups < 2 * kCus && steps >= 8)
-    x.splits = (int)std::min<int64_t>(std::min<int64_t>((2 * kCus + groups - 1) / std::max<int64_t>(groups, 1), steps / 4),
+  const int64_t want = (p.few ? 8 : 2) * kCus;
+  if (groups < want && steps >= 8)
+    x.splits = (int)std::min<int64_t>(std::min<int64_t>((want + groups - 1) / std::max<int64_t>(groups, 1), steps / 4),
                                       kMaxSplits);
   x.splits = std::max(x.splits, 1);
   if (x.splits > 1) p.work = up(4LL * x.splits * a.nq * a.heads * a.dim) + up(8LL * x.splits * a.nq * a.heads);

@@ -37,7 +37,7 @@ struct DqShape {
   static constexpr int WAVES = 4, THREADS = 256, ROWS = 128;
   static constexpr int BK = 32;
   typedef Tile<T, DT, BK, THREADS> KV;
-  static constexpr int DOCS = 4 * KV::BYTES, BIAS = DOCS + 2 * 4 * BK;
+  static constexpr int DOCS = 4 * KV::BYTES, LIVE = DOCS + 2 * 4 * BK, BIAS = LIVE + 16 * kDocWords;
 };
 
 template <class T, int DT, int FEAT>
@@ -51,10 +51,11 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : 2) void attend_dq_kernel(
   const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   int *const kdocs = (int *)(smem + Sh::DOCS);
+  uint64_t *const live = (uint64_t *)(smem + Sh::LIVE), *const pure = live + kDocWords;
   float *const bias = (float *)(smem + Sh::BIAS);
-  // sums of dZ by distance, an array each half of a wave
-  const int span = 2 * a.reach + 1;
-  float *const dist = bias + attend_bias_len(a.reach);
+  // sums of dZ by distance, an array each half of a wave, with the bias' ends
+  const int span = 2 * a.reach + 1, len = attend_bias_len(a.reach);
+  float *const dist = bias + len;
 
   const int head = blockIdx.x % a.heads, kvh = head / x.group;
   const int64_t slot = x.slots - 1 - blockIdx.x / a.heads;
@@ -120,10 +121,14 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : 2) void attend_dq_kernel(
   if constexpr (FEAT & kBias) {
     if (a.table) load_bias<T>(a, head, bias, tid, THREADS);
     if (grad_table)
-      for (int i = tid; i < 2 * Sh::WAVES * span; i += THREADS) dist[i] = 0.0f;
-    __syncthreads();
+      for (int i = tid; i < 2 * Sh::WAVES * len; i += THREADS) dist[i] = 0.0f;
   }
-  float *const my_dist = dist + (2 * wave + h) * span;
+  if (a.q_docs)
+    doc_steps<BK, Sh::WAVES>(a.q_docs + s.q0, first, min(first + ROWS, s.nq) - 1, a.k_docs + s.k0, s.nk, t_begin, t_end,
+                             live, pure, wave, lane);
+  if (a.q_docs || (FEAT & kBias)) __syncthreads();
+  auto next = [&](int t) { return a.q_docs ? next_live(live, t, t_begin, t_end) : t; };
+  float *const my_dist = dist + (2 * wave + h) * len;
   float below = 0.0f, above = 0.0f;  // dZ at distances of -reach and less, reach and more
 
   v16f acc[ND];
@@ -135,25 +140,28 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : 2) void attend_dq_kernel(
   auto fetch = [&](int t) {
     kt.get(kb, a.k.row, t * BK, s.nk, a.dim, tid);
     vt.get(vb, a.v.row, t * BK, s.nk, a.dim, tid);
-    if (a.q_docs && tid < BK) kdoc = t * BK + tid < s.nk ? a.k_docs[s.k0 + t * BK + tid] : -1;
+    if (a.q_docs) {
+      kt.get_tags(a.k_docs + s.k0, t * BK, s.nk, tid);
+      if (tid < BK) kdoc = a.k_docs[s.k0 + min(t * BK + tid, s.nk - 1)];
+    }
   };
-  int buf = 0;
-  if (t_begin < t_end) fetch(t_begin);
-  for (int t = t_begin; t < t_end; t++, buf ^= 1) {
+  int buf = 0, t = next(t_begin);
+  if (t < t_end) fetch(t);
+  for (int tn; t < t_end; t = tn, buf ^= 1) {
     char *const kl = smem + buf * 2 * KV::BYTES, *const vl = kl + KV::BYTES;
-    const bool docs = a.q_docs != nullptr;
+    const bool docs = a.q_docs && !is_pure(pure, t - t_begin);
     {
       const bool all = a.dim == DT && t * BK + BK <= s.nk && !docs;
-      if (docs) {
-        if (tid < BK) kdocs[buf * BK + tid] = kdoc < 0 ? -2 : kdoc;
-        __syncthreads();
-      }
-      auto keep = [&](int r) { return t * BK + r < s.nk && (!docs || kdocs[buf * BK + r] >= 0); };
-      kt.put(kl, a.dim, tid, all, keep);
-      vt.put(vl, a.dim, tid, all, keep);
+      auto keep = [&](int d) { return !docs || d >= 0; };
+      if (docs && tid < BK) kdocs[buf * BK + tid] = kdoc < 0 ? -2 : kdoc;
+      kt.put(kl, s.nk - t * BK, a.dim, tid, all, keep);
+#pragma unroll
+      for (int i = 0; i < KV::N; i++) vt.tag[i] = kt.tag[i];
+      vt.put(vl, s.nk - t * BK, a.dim, tid, all, keep);
     }
     __syncthreads();
-    if (t + 1 < t_end) fetch(t + 1);
+    tn = next(t + 1);
+    if (tn < t_end) fetch(tn);
     const int j0 = t * BK;
     if (j0 > hi_max || j0 + BK <= lo_min) continue;
 
@@ -219,17 +227,10 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : 2) void attend_dq_kernel(
           // register by register: the 32 queries of a half have 32 distances
           // to one key, so no two lanes add to one place, and a wave's adds
           // to its own arrays keep their order
+          typedef __attribute__((address_space(3))) float lfloat;
+          lfloat *const at = (lfloat *)(my_dist + d0 + a.reach + kBiasPad);
 #pragma unroll
-          for (int r = 0; r < 16; r++) {
-            const int d = d0 + 8 * (r >> 2) + (r & 3);
-            if (d >= a.reach)
-              above += dz[r];
-            else if (d <= -a.reach)
-              below += dz[r];
-            else
-              __builtin_amdgcn_ds_faddf((__attribute__((address_space(3))) float *)(my_dist + d + a.reach), dz[r], 0, 0,
-                                        false);
-          }
+          for (int r = 0; r < 16; r++) __builtin_amdgcn_ds_faddf(at + 8 * (r >> 2) + (r & 3), dz[r], 0, 0, false);
         }
       }
     }
@@ -260,22 +261,29 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : 2) void attend_dq_kernel(
   }
   if constexpr (FEAT & kBias) {
     if (grad_table) {
-      // the ends: every lane's sums, in a fixed order of the lanes
+      // the ends: the lanes' sums in a fixed order, then the arrays past the
+      // reach, which are the ends' too
 #pragma unroll
       for (int o = 1; o < 64; o <<= 1) {
         above += __shfl_xor(above, o);
         below += __shfl_xor(below, o);
       }
-      if (lane == 0) {
-        float *const d = dist + 2 * wave * span;
-        d[0] = below;
-        d[span - 1] = above;
+      float *const d = dist + 2 * wave * len;
+      if (lane == 0) d[0] += below, d[len - 1] += above;
+      __syncthreads();
+      for (int i = tid; i < len; i += THREADS) {
+        float v = 0.0f;
+#pragma unroll
+        for (int w = 0; w < 2 * Sh::WAVES; w++) v += dist[w * len + i];
+        dist[i] = v;
       }
       __syncthreads();
       for (int i = tid; i < span; i += THREADS) {
-        float v = 0.0f;
-#pragma unroll
-        for (int w = 0; w < 2 * Sh::WAVES; w++) v += dist[w * span + i];
+        float v = dist[i + kBiasPad];
+        if (i == 0)
+          for (int e = 0; e < kBiasPad; e++) v += dist[e];
+        if (i == span - 1)
+          for (int e = 1; e <= kBiasPad; e++) v += dist[i + kBiasPad + e];
         dist_out[i] = v;
       }
     }
@@ -290,7 +298,8 @@ struct DkvShape {
   static constexpr int BQ = 32;
   typedef Tile<T, DT, BQ, THREADS> QO;
   // Q and dO twice, then lse, delta and the documents of the rows twice
-  static constexpr int STAT = 4 * QO::BYTES, DOCS = STAT + 4 * 4 * BQ, BIAS = DOCS + 2 * 4 * BQ;
+  static constexpr int STAT = 4 * QO::BYTES, DOCS = STAT + 4 * 4 * BQ, LIVE = DOCS + 2 * 4 * BQ,
+                       BIAS = LIVE + 16 * kDocWords;
 };
 
 template <class T, int DT, int FEAT>
@@ -305,6 +314,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 || DT == 128 ? 1 : 2) void atte
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   float *const stat = (float *)(smem + Sh::STAT);
   int *const qdocs = (int *)(smem + Sh::DOCS);
+  uint64_t *const live = (uint64_t *)(smem + Sh::LIVE), *const pure = live + kDocWords;
   float *const bias = (float *)(smem + Sh::BIAS);
 
   const int kvh = blockIdx.x % a.kv_heads;
@@ -349,6 +359,13 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 || DT == 128 ? 1 : 2) void atte
       v[i] = load8(vr + 16 * i + 8 * h, in);
     }
   }
+  if (a.q_docs) {
+    doc_steps<BQ, Sh::WAVES>(a.k_docs + s.k0, first, min(first + KEYS, s.nk) - 1, a.q_docs + s.q0, s.nq, t_begin, t_end,
+                             live, pure, wave, lane);
+    __syncthreads();
+  }
+  auto next = [&](int t) { return a.q_docs ? next_live(live, t, t_begin, t_end) : t; };
+  const int t_first = next(t_begin);
   const Score sc(a, FEAT & kCap);
   v16f dk[ND], dv[ND];
 #pragma unroll
@@ -373,31 +390,37 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 || DT == 128 ? 1 : 2) void atte
     auto fetch = [&](int t) {
       qt.get(qb, a.q.row, t * BQ, s.nq, a.dim, tid);
       gt.get(gb, x.g.d_out.row, t * BQ, s.nq, a.dim, tid);
+      // a row that sees nothing has lse -inf
+      qt.get_tags((const int32_t *)lse_of, t * BQ, s.nq, tid);
       if (tid < BQ) {
-        const int r = t * BQ + tid;
-        lse = r < s.nq ? lse_of[r] : -INFINITY;
-        delta = r < s.nq ? delta_of[r] : 0.0f;
-        if (a.q_docs) qdoc = r < s.nq ? max(a.q_docs[s.q0 + r], -1) : -1;
+        const int r = min(t * BQ + tid, s.nq - 1);
+        lse = lse_of[r];
+        delta = delta_of[r];
+        if (a.q_docs) qdoc = a.q_docs[s.q0 + r];
       }
     };
-    if (t_begin < t_end) fetch(t_begin);
-    for (int t = t_begin; t < t_end; t++, buf ^= 1) {
+    if (t_first < t_end) fetch(t_first);
+    for (int t = t_first, tn; t < t_end; t = tn, buf ^= 1) {
       char *const ql = smem + buf * 2 * QO::BYTES, *const gl = ql + QO::BYTES;
       float *const st = stat + buf * 2 * BQ;
+      const bool docs = a.q_docs && !is_pure(pure, t - t_begin);
       {
-        // a row that sees nothing (lse -inf) is cleared: P is 0 at +inf
+        // such rows, and those past the last, are cleared: P is 0 at +inf
         if (tid < BQ) {
-          st[tid] = lse > -INFINITY ? lse * kLog2e : INFINITY;
-          st[BQ + tid] = lse > -INFINITY ? delta : 0.0f;
-          qdocs[buf * BQ + tid] = qdoc;
+          const bool there = lse > -INFINITY && t * BQ + tid < s.nq;
+          st[tid] = there ? lse * kLog2e : INFINITY;
+          st[BQ + tid] = there ? delta : 0.0f;
+          qdocs[buf * BQ + tid] = max(qdoc, -1);
         }
-        __syncthreads();
-        auto keep = [&](int r) { return st[r] < INFINITY; };
-        qt.put(ql, a.dim, tid, false, keep);
-        gt.put(gl, a.dim, tid, false, keep);
+        auto keep = [&](int l) { return __builtin_bit_cast(float, l) > -INFINITY; };
+        qt.put(ql, s.nq - t * BQ, a.dim, tid, false, keep);
+#pragma unroll
+        for (int i = 0; i < QO::N; i++) gt.tag[i] = qt.tag[i];
+        gt.put(gl, s.nq - t * BQ, a.dim, tid, false, keep);
       }
       __syncthreads();
-      if (t + 1 < t_end) fetch(t + 1);
+      tn = next(t + 1);
+      if (tn < t_end) fetch(tn);
       const int p0 = t * BQ + s.shift;  // place of the step's first query
       if (p0 > hi_max || p0 + BQ <= lo_min) continue;
 
@@ -437,12 +460,12 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 || DT == 128 ? 1 : 2) void atte
 #pragma unroll
         for (int e = 0; e < 4; e++) pr[4 * g4 + e] = exp2_fast(z[4 * g4 + e] - l[e]);
       }
-      if (a.q_docs || p0 < lo_max || p0 + BQ - 1 > hi_min) {
+      if (docs || p0 < lo_max || p0 + BQ - 1 > hi_min) {
         const unsigned e0 = p0 + 4 * h - lo;
 #pragma unroll
         for (int r = 0; r < 16; r++)
           if (e0 + (unsigned)(8 * (r >> 2) + (r & 3)) > width) pr[r] = 0.0f;
-        if (a.q_docs) {
+        if (docs) {
 #pragma unroll
           for (int g4 = 0; g4 < 4; g4++) {
             const i4 d = *(const i4 *)(qdocs + buf * BQ + 8 * g4 + 4 * h);
@@ -511,12 +534,13 @@ __global__ __launch_bounds__(256) void attend_dist_kernel(AttendArgs x) {
         (strand[0][threadIdx.x] + strand[1][threadIdx.x]) + (strand[2][threadIdx.x] + strand[3][threadIdx.x]);
 }
 
-// The distances of each bucket: a block a head, the bucket's distances in
-// ascending order.
+// The distances of each bucket: a block a head, 256 / n_buckets strands a
+// bucket (at least one), each of its distances in ascending order.
 template <class T>
 __global__ __launch_bounds__(256) void attend_dtable_kernel(AttendArgs x) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  const int span = 2 * x.a.reach + 1, head = blockIdx.x;
+  __shared__ float strand[256];
+  const int span = 2 * x.a.reach + 1, head = blockIdx.x, nb = x.a.n_buckets;
   float *const sum = (float *)smem;
   int *const of = (int *)(sum + span);
   for (int i = threadIdx.x; i < span; i += 256) {
@@ -526,10 +550,20 @@ __global__ __launch_bounds__(256) void attend_dtable_kernel(AttendArgs x) {
     of[i] = x.a.buckets[i];
   }
   __syncthreads();
-  for (int b = threadIdx.x; b < x.a.n_buckets; b += 256) {
+  const int strands = max(256 / nb, 1), per = (span + strands - 1) / strands;
+  const int w = nb < 256 ? threadIdx.x / nb : 0;
+  for (int b0 = 0; b0 < nb; b0 += 256) {
+    const int b = b0 + (nb < 256 ? threadIdx.x % nb : threadIdx.x);
     float v = 0.0f;
-    for (int i = 0; i < span; i++) v += of[i] == b ? sum[i] : 0.0f;
-    ((T *)x.g.dtable)[(int64_t)b * x.a.heads + head] = (T)v;
+    if (b < nb && w < strands)
+      for (int i = w * per; i < min(span, (w + 1) * per); i++) v += of[i] == b ? sum[i] : 0.0f;
+    strand[threadIdx.x] = v;
+    __syncthreads();
+    if (w == 0 && b < nb) {
+      for (int i = 1; i < strands; i++) v += strand[i * nb + b];
+      ((T *)x.g.dtable)[(int64_t)b * x.a.heads + head] = (T)v;
+    }
+    __syncthreads();
   }
 }
 
@@ -537,7 +571,7 @@ template <class T, int DT, int FEAT>
 bool run_dq(const AttendArgs &x, hipStream_t s) {
   typedef DqShape<T, DT> Sh;
   const int len = (FEAT & kBias) && x.a.table ? attend_bias_len(x.a.reach) : 0;
-  const int shm = Sh::BIAS + 4 * len + (len ? 8 * 4 * (2 * x.a.reach + 1) : 0);
+  const int shm = Sh::BIAS + 4 * len * (1 + 2 * Sh::WAVES);
   static PerDevice lds;
   if (!lds_granted(lds, (const void *)attend_dq_kernel<T, DT, FEAT>, 160 << 10)) return false;
   attend_dq_kernel<T, DT, FEAT><<<dim3((unsigned)(x.slots * x.a.heads)), Sh::THREADS, shm, s>>>(x);

@@ -145,6 +145,7 @@ struct Tile {
   static constexpr int N = R * CH / THREADS;       // pieces a thread
   static_assert(N * THREADS == R * CH && CH >= 8, "");
   i4 part[N];
+  int tag[N];
 
   // Starts the loads of rows r0.. of the sequence (n rows in all, from base):
   // a row past the last and a piece past `dim` are read where there is one
@@ -158,14 +159,20 @@ struct Tile {
       part[i] = *(const i4 *)(base + row * stride + col);
     }
   }
-  // Writes them. keep(r): whether row r of the tile is used; others are 0.
+  // Starts the loads of those rows' tags, by which put() may drop them too.
+  __device__ __forceinline__ void get_tags(const int32_t *base, int r0, int n, int tid) {
+#pragma unroll
+    for (int i = 0; i < N; i++) tag[i] = base[min(r0 + (tid + i * THREADS) / CH, n - 1)];
+  }
+  // Writes them; what is past `rows` rows or `dim` columns, and rows whose
+  // tag keep() refuses, as 0. all: nothing is.
   template <class Keep>
-  __device__ __forceinline__ void put(char *lds, int dim, int tid, bool all, Keep keep) {
+  __device__ __forceinline__ void put(char *lds, int rows, int dim, int tid, bool all, Keep keep) {
 #pragma unroll
     for (int i = 0; i < N; i++) {
       const int at = tid + i * THREADS, r = at / CH, c = at % CH;
       i4 v = part[i];
-      if (!all && !(c * EPC < dim && keep(r))) v = i4{0, 0, 0, 0};
+      if (!all && !(c * EPC < dim && r < rows && keep(tag[i]))) v = i4{0, 0, 0, 0};
       *(i4 *)(lds + r * RB + ((c ^ (r & 7)) << 4)) = v;
     }
   }
@@ -273,6 +280,66 @@ __device__ __forceinline__ void query_bounds(const ixh_attend_args &a, const Seq
   }
   *lo = l;
   *hi = h;
+}
+
+// ---- documents --------------------------------------------------------------
+
+constexpr int kDocWords = 64;  // of 64 steps; later steps are taken as live
+
+// Which of the steps t0..t1 - 1 (`step` rows each, of the n in `theirs`) hold
+// a row of a document that a row first..last of `mine` has, and which hold
+// one document alone, that of all of mine (pure: no mask is needed). Every
+// wave calls it; a barrier before the words are read.
+template <int STEP, int WAVES>
+__device__ __forceinline__ void doc_steps(const int32_t *mine, int first, int last, const int32_t *theirs, int n, int t0,
+                                          int t1, uint64_t *live, uint64_t *pure, int wave, int lane) {
+  int mn = INT32_MAX, mx = -1;
+  bool none = false;
+  for (int i = first + lane; i <= last; i += 64) {
+    const int d = mine[i];
+    none |= d < 0;
+    mn = min(mn, d < 0 ? INT32_MAX : d);
+    mx = max(mx, d);
+  }
+#pragma unroll
+  for (int o = 32; o; o >>= 1) {
+    mn = min(mn, __shfl_xor(mn, o));
+    mx = max(mx, __shfl_xor(mx, o));
+  }
+  const bool one = mn == mx && !__ballot(none);
+  for (int w = wave; w < kDocWords && t0 + 64 * w < t1; w += WAVES) {
+    const int t = t0 + 64 * w + lane;
+    int tmn = INT32_MAX, tmx = -1;
+    bool bad = t >= t1 || t * STEP + STEP > n;
+    if (t < t1) {
+#pragma unroll
+      for (int i = 0; i < STEP; i++) {
+        const int d = theirs[min(t * STEP + i, n - 1)];
+        bad |= d < 0;
+        tmn = min(tmn, d < 0 ? INT32_MAX : d);
+        tmx = max(tmx, d);
+      }
+    }
+    const bool some = tmx >= 0 && mx >= 0 && tmn <= mx && tmx >= mn;
+    const uint64_t lv = __ballot(some), pr = __ballot(some && one && !bad && tmn == tmx && tmn == mn);
+    if (lane == 0) live[w] = lv, pure[w] = pr;
+  }
+}
+// The first live step from t on, t1 if none.
+__device__ __forceinline__ int next_live(const uint64_t *live, int t, int t0, int t1) {
+  while (t < t1) {
+    const int i = t - t0;
+    if (i >= 64 * kDocWords) return t;
+    const uint64_t w = live[i >> 6] >> (i & 63);
+    const int skip = __builtin_amdgcn_readfirstlane(w ? __builtin_ctzll(w) : 64 - (i & 63));
+    const bool hit = __builtin_amdgcn_readfirstlane(w != 0);
+    t += skip;
+    if (hit) return min(t, t1);
+  }
+  return t1;
+}
+__device__ __forceinline__ bool is_pure(const uint64_t *pure, int i) {
+  return i < 64 * kDocWords && __builtin_amdgcn_readfirstlane((int)(pure[i >> 6] >> (i & 63)) & 1);
 }
 
 // ---- scores -----------------------------------------------------------------

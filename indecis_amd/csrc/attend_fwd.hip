@@ -13,8 +13,6 @@
 namespace ixh {
 namespace {
 
-constexpr int kDocWords = 64;  // 64 steps of keys a word; later steps are taken as live
-
 template <class T, int DT, int WAVES>
 struct FwdShape {
   static constexpr int THREADS = 64 * WAVES, ROWS = 32 * WAVES;
@@ -85,40 +83,8 @@ __global__ __launch_bounds__(64 * WAVES, 2) void attend_fwd_kernel(AttendArgs x)
   int doc = 0;
   if (a.q_docs) {
     doc = max(a.q_docs[s.q0 + tok], -1);
-    // over the workgroup's rows
-    const int first = (int)(blk * ROWS / pack), last = (int)((min(blk * ROWS + ROWS, rows) - 1) / pack);
-    int all_mn = INT32_MAX, all_mx = -1;
-    bool none = false;
-    for (int i = first + (lane & 31); i <= last; i += 32) {
-      const int d = a.q_docs[s.q0 + i];
-      none |= d < 0;
-      all_mn = min(all_mn, d < 0 ? INT32_MAX : d);
-      all_mx = max(all_mx, d);
-    }
-#pragma unroll
-    for (int o = 16; o; o >>= 1) {
-      all_mn = min(all_mn, __shfl_xor(all_mn, o));
-      all_mx = max(all_mx, __shfl_xor(all_mx, o));
-    }
-    const bool one = all_mn == all_mx && !__ballot(none);
-    for (int w = wave; w < kDocWords && t_begin + 64 * w < t_end; w += WAVES) {
-      const int t = t_begin + 64 * w + lane;
-      int kmn = INT32_MAX, kmx = -1;
-      bool bad = t >= t_end || t * BK + BK > s.nk;
-      if (t < t_end) {
-        const int32_t *kd = a.k_docs + s.k0;
-#pragma unroll 32
-        for (int i = 0; i < BK; i++) {
-          const int d = kd[min(t * BK + i, s.nk - 1)];
-          bad |= d < 0;
-          kmn = min(kmn, d < 0 ? INT32_MAX : d);
-          kmx = max(kmx, d);
-        }
-      }
-      const bool some = kmx >= 0 && all_mx >= 0 && kmn <= all_mx && kmx >= all_mn;
-      const uint64_t lv = __ballot(some), pr = __ballot(some && one && !bad && kmn == kmx && kmn == all_mn);
-      if (lane == 0) live[w] = lv, pure[w] = pr;
-    }
+    doc_steps<BK, WAVES>(a.q_docs + s.q0, (int)(blk * ROWS / pack), (int)((min(blk * ROWS + ROWS, rows) - 1) / pack),
+                         a.k_docs + s.k0, s.nk, t_begin, t_end, live, pure, wave, lane);
   }
   if constexpr (FEAT & kBias) {
     if (a.table)
@@ -127,19 +93,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void attend_fwd_kernel(AttendArgs x)
   }
   if (a.q_docs || (FEAT & kBias)) __syncthreads();
 
-  auto next = [&](int t) {
-    if (!a.q_docs) return t;
-    while (t < t_end) {
-      const int i = t - t_begin;
-      if (i >= 64 * kDocWords) return t;
-      const uint64_t w = live[i >> 6] >> (i & 63);
-      const int skip = w ? __builtin_ctzll(w) : 64 - (i & 63);
-      const int n = __builtin_amdgcn_readfirstlane(skip);
-      t += n;
-      if (n == 0) return t;
-    }
-    return t_end;
-  };
+  auto next = [&](int t) { return a.q_docs ? next_live(live, t, t_begin, t_end) : t; };
 
   // Q's fragments, columns past dim 0
   Frag q[KS];
@@ -164,7 +118,10 @@ __global__ __launch_bounds__(64 * WAVES, 2) void attend_fwd_kernel(AttendArgs x)
   auto fetch = [&](int t) {
     kt.get(kb, a.k.row, t * BK, s.nk, a.dim, tid);
     vt.get(vb, a.v.row, t * BK, s.nk, a.dim, tid);
-    if (a.q_docs && tid < BK) kdoc = t * BK + tid < s.nk ? a.k_docs[s.k0 + t * BK + tid] : -1;
+    if (a.q_docs) {
+      kt.get_tags(a.k_docs + s.k0, t * BK, s.nk, tid);
+      if (tid < BK) kdoc = a.k_docs[s.k0 + min(t * BK + tid, s.nk - 1)];
+    }
   };
 
   int buf = 0;
@@ -172,17 +129,16 @@ __global__ __launch_bounds__(64 * WAVES, 2) void attend_fwd_kernel(AttendArgs x)
   if (t < t_end) fetch(t);
   while (t < t_end) {
     char *const kl = smem + buf * 2 * KV::BYTES, *const vl = kl + KV::BYTES;
-    const bool dead = a.q_docs && !(t - t_begin < 64 * kDocWords && (pure[(t - t_begin) >> 6] >> ((t - t_begin) & 63) & 1));
+    const bool docs = a.q_docs && !is_pure(pure, t - t_begin);
     {
-      // keys that no query sees hold anything: their rows are cleared
-      const bool all = a.dim == DT && t * BK + BK <= s.nk && !dead;
-      if (dead) {
-        if (tid < BK) kdocs[buf * BK + tid] = kdoc < 0 ? -2 : kdoc;
-        __syncthreads();
-      }
-      auto keep = [&](int row) { return t * BK + row < s.nk && (!dead || kdocs[buf * BK + row] >= 0); };
-      kt.put(kl, a.dim, tid, all, keep);
-      vt.put(vl, a.dim, tid, all, keep);
+      // padding that no query sees may hold anything: its rows are cleared
+      const bool all = a.dim == DT && t * BK + BK <= s.nk && !docs;
+      auto keep = [&](int d) { return !docs || d >= 0; };
+      if (docs && tid < BK) kdocs[buf * BK + tid] = kdoc < 0 ? -2 : kdoc;
+      kt.put(kl, s.nk - t * BK, a.dim, tid, all, keep);
+#pragma unroll
+      for (int i = 0; i < KV::N; i++) vt.tag[i] = kt.tag[i];
+      vt.put(vl, s.nk - t * BK, a.dim, tid, all, keep);
     }
     __syncthreads();
     const int tn = next(t + 1);
@@ -197,7 +153,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void attend_fwd_kernel(AttendArgs x)
 #pragma unroll
         for (int i = 0; i < KS; i++) z[u] = mfma16(KV::rows(kl, 32 * u, i, lane), q[i], z[u]);
       }
-      const bool masked = dead || j0 < lo_max || j0 + BK - 1 > hi_min;
+      const bool masked = docs || j0 < lo_max || j0 + BK - 1 > hi_min;
       if constexpr (FEAT != 0) {
 #pragma unroll
         for (int u = 0; u < NS; u++) {
@@ -241,7 +197,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void attend_fwd_kernel(AttendArgs x)
 #pragma unroll
           for (int r = 0; r < 16; r++)
             if (e0 + (unsigned)(8 * (r >> 2) + (r & 3)) > width) z[u][r] = -INFINITY;
-          if (dead) {
+          if (docs) {
 #pragma unroll
             for (int g = 0; g < 4; g++) {
               const i4 d = *(const i4 *)(kdocs + buf * BK + 32 * u + 8 * g + 4 * h);

@@ -248,27 +248,30 @@ __global__ __launch_bounds__(kThreads) void norm_rope_backward_kernel(NormRopeAr
   }
 }
 
-// A block has 16 columns of one gamma, 16 strands of the parts each.
+// A block has 4 columns of one gamma, a thread every 256th part of them.
 __global__ __launch_bounds__(256) void norm_rope_gamma_kernel(NormRopeArgs x, int parts) {
-  __shared__ float strand[16][17];
+  __shared__ f4 strand[4];
   const ixh_norm_rope_args &a = x.a;
-  const int c = blockIdx.x * 16 + (threadIdx.x & 15), w = threadIdx.x >> 4;
+  const int c = blockIdx.x * 4;
   void *const to = blockIdx.y ? x.g.dk_gamma : x.g.dq_gamma;
   if (!to) return;
-  float v = 0.0f;
-  if (c < a.dim)
-    for (int i = w; i < parts; i += 16) v += x.part[((int64_t)i * 2 + blockIdx.y) * a.dim + c];
-  strand[w][threadIdx.x & 15] = v;
+  f4 v{};
+#pragma unroll 4
+  for (int i = threadIdx.x; i < parts; i += 256) v += *(const f4 *)(x.part + ((int64_t)i * 2 + blockIdx.y) * a.dim + c);
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1)
+#pragma unroll
+    for (int e = 0; e < 4; e++) v[e] += __shfl_xor(v[e], o);
+  if (threadIdx.x % 64 == 0) strand[threadIdx.x / 64] = v;
   __syncthreads();
-  if (w || c >= a.dim) return;
-  v = 0.0f;
-  for (int i = 0; i < 16; i++) v += strand[i][threadIdx.x];
+  if (threadIdx.x) return;
+  v = (strand[0] + strand[1]) + (strand[2] + strand[3]);
   if (a.gamma_type == IXH_TYPE_F32)
-    ((float *)to)[c] = v;
+    store4((float *)to + c, v);
   else if (a.gamma_type == IXH_TYPE_BF16)
-    ((__bf16 *)to)[c] = (__bf16)v;
+    store4((__bf16 *)to + c, v);
   else
-    ((_Float16 *)to)[c] = (_Float16)v;
+    store4((_Float16 *)to + c, v);
 }
 
 template <class T, int LANES, int NORM>
@@ -309,7 +312,7 @@ void launch_norm_rope_backward(const NormRopeArgs &x, hipStream_t s) {
   by_type(x, true, s);
   if (!x.part) return;
   const int steps = (x.a.q_heads + x.a.k_heads + x.heads_step - 1) / x.heads_step;
-  norm_rope_gamma_kernel<<<dim3((x.a.dim + 15) / 16, 2), 256, 0, s>>>(x, x.blocks * steps);
+  norm_rope_gamma_kernel<<<dim3(x.a.dim / 4, 2), 256, 0, s>>>(x, x.blocks * steps);
 }
 
 }  // namespace ixh
