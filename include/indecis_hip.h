@@ -404,8 +404,8 @@ int ixh_attend8(int device, float *o, const float *q, const float *k,
 enum { IXH_TYPE_F32 = 0, IXH_TYPE_BF16 = 1, IXH_TYPE_F16 = 2 };
 
 /* Rows of heads in device memory: value i of a head of a row stands at
- * p[row * r + head * h + i], in values of the call's type. p and both
- * strides are multiples of 16 bytes. */
+ * p[r * row + h * head + i], in values of the call's type. p and both
+ * strides are multiples of 16 bytes, the rows less than 2^27 bytes apart. */
 typedef struct ixh_heads {
   void *p;
   int64_t row, head;
@@ -420,8 +420,8 @@ typedef struct ixh_attend_args {
   ixh_heads q, k, v, o;  /* [nq][heads][dim], [nk][kv_heads][dim] twice, [nq][heads][dim] */
   const int32_t *q_offs; /* [B+1]: rows of each sequence's queries, ascending */
   const int32_t *k_offs; /* [B+1] of its keys; NULL: q_offs, and nk == nq */
-  float scale;           /* of the products, > 0 */
-  float cap;             /* > 0: scores become cap * tanh(score / cap); 0: not */
+  float scale;           /* of the products, 1e-10 to 1e10 */
+  float cap;             /* 1e-10 to 1e10: scores become cap * tanh(score / cap); 0: not */
   const float *slopes;   /* [heads]: score -= slope * distance; NULL: none */
   const void *table;     /* [n_buckets][heads]: score += table[bucket][head]; NULL: none */
   const int32_t *buckets; /* [2 reach + 1]: the bucket of distance -reach..reach (key less

@@ -56,10 +56,11 @@ int64_t up(int64_t n) { return (n + 255) / 256 * 256; }
 int check_heads(const char *op, const char *name, const ixh_heads &t, int type) {
   const int v = 16 / type_size(type);
   if (!t.p) return fail(IXH_EINVAL, "linalg: %s: %s is missing", op, name);
-  if (!aligned(t.p) || t.row % v || t.head % v)
+  // a thread's place in a tile of rows is a 32-bit offset: 32 rows
+  if (!aligned(t.p) || t.row % v || t.head % v || t.row < 0 || t.head < 0 || t.row >= (1LL << 27) / type_size(type))
     return fail(IXH_EINVAL,
-                "linalg: %s: %s needs a pointer and strides that are multiples of 16 bytes (strides %lld, %lld values "
-                "of %d bytes)",
+                "linalg: %s: %s needs a pointer and strides that are multiples of 16 bytes, rows less than 2^27 bytes "
+                "apart (strides %lld, %lld values of %d bytes)",
                 op, name, (long long)t.row, (long long)t.head, type_size(type));
   return IXH_OK;
 }
@@ -92,8 +93,11 @@ int check_sizes(const ixh_attend_args *a) {
 
 int check_attend(const ixh_attend_args *a) {
   if (int rc = check_sizes(a)) return rc;
-  if (!(a->scale > 0) || !std::isfinite(a->scale) || !(a->cap >= 0) || !std::isfinite(a->cap))
-    return fail(IXH_EINVAL, "linalg: Attend: scale %g (above 0), cap %g (0 or above)", (double)a->scale, (double)a->cap);
+  // a bias is taken in units of 1 / scale, a capped score in units of cap
+  const bool scale_ok = a->scale >= 1e-10f && a->scale <= 1e10f, cap_ok = a->cap == 0 || (a->cap >= 1e-10f && a->cap <= 1e10f);
+  if (!scale_ok || !cap_ok)
+    return fail(IXH_EINVAL, "linalg: Attend: scale %g (1e-10 to 1e10), cap %g (the same, or 0)", (double)a->scale,
+                (double)a->cap);
   if (a->prefix && !a->causal) return fail(IXH_EINVAL, "linalg: Attend: a prefix needs causal");
   if (a->B == 0) return IXH_OK;
   if (!a->q_offs) return fail(IXH_EINVAL, "linalg: Attend: q_offs is missing");

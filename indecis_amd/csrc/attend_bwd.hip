@@ -15,15 +15,16 @@
 namespace ixh {
 namespace {
 
-// z and its derivative by the score where there is a cap, for 16 scores.
+// z (base 2) of 16 scores, and under a cap its derivative by the score.
 template <class T, int FEAT>
-__device__ __forceinline__ void shape_scores(v16f &z, float *slope_of, const Score &sc) {
+__device__ __forceinline__ void shape_scores(v16f &z, float *slope_of, const Score &sc, const Bias &by, const v16f &bias) {
 #pragma unroll
   for (int r = 0; r < 16; r++) {
     if constexpr (FEAT & kCap) {
       float u;
-      z[r] = sc.c2 * tanh_of<T>(z[r] * sc.c1, &u);
+      z[r] = capped<T>(sc, z[r], &u);
       slope_of[r] = 4.0f * u * (1.0f - u);
+      if constexpr (FEAT & kBias) z[r] += bias[r];
     } else {
       z[r] *= sc.c1;
     }
@@ -53,7 +54,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : 2) void attend_dq_kernel(
   int *const kdocs = (int *)(smem + Sh::DOCS);
   uint64_t *const live = (uint64_t *)(smem + Sh::LIVE), *const pure = live + kDocWords;
   float *const bias = (float *)(smem + Sh::BIAS);
-  // sums of dZ by distance, an array each half of a wave, with the bias' ends
+  // sums of dZ by distance, an array each wave, with the bias' ends
   const int span = 2 * a.reach + 1, len = attend_bias_len(a.reach);
   float *const dist = bias + len;
 
@@ -78,9 +79,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : 2) void attend_dq_kernel(
   key_bounds(a, s, p, &lo, &hi);
   const int p_lo = __builtin_amdgcn_readlane(p, 0), p_hi = __builtin_amdgcn_readlane(p, 31);
   const int lo_min = __builtin_amdgcn_readlane(lo, 0), lo_max = __builtin_amdgcn_readlane(lo, 31);
-  const int hi_min = __builtin_amdgcn_readlane(hi, 0), hi_max = __builtin_amdgcn_readlane(hi, 31);
-  if (hi < lo) lo = 1 << 30, hi = 1 << 30;
-  const unsigned width = hi - lo;
+  const int hi_min = __builtin_amdgcn_readlane(hi, 0);
+  const int hi_max = first + wave * 32 < s.nq ? __builtin_amdgcn_readlane(hi, 31) : -1;
   int t_begin, t_end;
   {
     int l, u, unused;
@@ -117,18 +117,20 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : 2) void attend_dq_kernel(
   const T *const kb = (const T *)a.k.p + s.k0 * a.k.row + kvh * a.k.head;
   const T *const vb = (const T *)a.v.p + s.k0 * a.v.row + kvh * a.v.head;
   const Score sc(a, FEAT & kCap);
-  const float slope = (FEAT & kBias) && a.slopes ? -a.slopes[head] * kLog2e : 0.0f;
+  const float unit = bias_unit(a, FEAT & kCap);
+  const Bias by{(FEAT & kBias) && a.table ? bias : nullptr,
+                (FEAT & kBias) && a.slopes ? -a.slopes[head] * unit : 0.0f, a.reach};
   if constexpr (FEAT & kBias) {
-    if (a.table) load_bias<T>(a, head, bias, tid, THREADS);
+    if (a.table) load_bias<T>(a, head, unit, bias, tid, THREADS);
     if (grad_table)
-      for (int i = tid; i < 2 * Sh::WAVES * len; i += THREADS) dist[i] = 0.0f;
+      for (int i = tid; i < Sh::WAVES * len; i += THREADS) dist[i] = 0.0f;
   }
   if (a.q_docs)
     doc_steps<BK, Sh::WAVES>(a.q_docs + s.q0, first, min(first + ROWS, s.nq) - 1, a.k_docs + s.k0, s.nk, t_begin, t_end,
                              live, pure, wave, lane);
   if (a.q_docs || (FEAT & kBias)) __syncthreads();
   auto next = [&](int t) { return a.q_docs ? next_live(live, t, t_begin, t_end) : t; };
-  float *const my_dist = dist + (2 * wave + h) * len;
+  float *const my_dist = dist + wave * len;
   float below = 0.0f, above = 0.0f;  // dZ at distances of -reach and less, reach and more
 
   v16f acc[ND];
@@ -136,13 +138,17 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : 2) void attend_dq_kernel(
   for (int d = 0; d < ND; d++) acc[d] = v16f{};
 
   KV kt, vt;
+  typename KV::Tags tags;
   int kdoc = 0;
+  kt.init(a.k.row, a.dim, tid);
+  vt.init(a.v.row, a.dim, tid);
   auto fetch = [&](int t) {
-    kt.get(kb, a.k.row, t * BK, s.nk, a.dim, tid);
-    vt.get(vb, a.v.row, t * BK, s.nk, a.dim, tid);
+    const int left = s.nk - t * BK;
+    kt.get(kb + (int64_t)(t * BK) * a.k.row, a.k.row, left, tid);
+    vt.get(vb + (int64_t)(t * BK) * a.v.row, a.v.row, left, tid);
     if (a.q_docs) {
-      kt.get_tags(a.k_docs + s.k0, t * BK, s.nk, tid);
-      if (tid < BK) kdoc = a.k_docs[s.k0 + min(t * BK + tid, s.nk - 1)];
+      tags.get(a.k_docs + s.k0 + t * BK, left, tid);
+      if (tid < BK) kdoc = a.k_docs[s.k0 + t * BK + min(tid, left - 1)];
     }
   };
   int buf = 0, t = next(t_begin);
@@ -154,10 +160,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : 2) void attend_dq_kernel(
       const bool all = a.dim == DT && t * BK + BK <= s.nk && !docs;
       auto keep = [&](int d) { return !docs || d >= 0; };
       if (docs && tid < BK) kdocs[buf * BK + tid] = kdoc < 0 ? -2 : kdoc;
-      kt.put(kl, s.nk - t * BK, a.dim, tid, all, keep);
-#pragma unroll
-      for (int i = 0; i < KV::N; i++) vt.tag[i] = kt.tag[i];
-      vt.put(vl, s.nk - t * BK, a.dim, tid, all, keep);
+      kt.put(kl, s.nk - t * BK, a.dim, tid, all, tags, keep);
+      vt.put(vl, s.nk - t * BK, a.dim, tid, all, tags, keep);
     }
     __syncthreads();
     tn = next(t + 1);
@@ -165,44 +169,26 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : 2) void attend_dq_kernel(
     const int j0 = t * BK;
     if (j0 > hi_max || j0 + BK <= lo_min) continue;
 
-    v16f z = v16f{}, dp = v16f{};
+    const int d0 = j0 + 4 * h - p;
+    const int near = j0 - p_hi, far = j0 + 31 - p_lo;
+    const bool flat = near >= a.reach || far <= -a.reach;
+    v16f z = v16f{}, dp = v16f{}, bz = v16f{};
+    if constexpr (FEAT & kBias) bz = by.template at<1>(d0, near, far);
+    if constexpr (FEAT == kBias) z = bz;
 #pragma unroll
     for (int i = 0; i < KS; i++) {
       z = mfma16(KV::rows(kl, 0, i, lane), q[i], z);
       dp = mfma16(KV::rows(vl, 0, i, lane), dO[i], dp);
     }
     float by_cap[16];
-    shape_scores<T, FEAT>(z, by_cap, sc);
-    const int d0 = j0 + 4 * h - p;
-    const int near = j0 - p_hi, far = j0 + 31 - p_lo;
-    const bool flat = near >= a.reach || far <= -a.reach;
-    if constexpr (FEAT & kBias) {
-      if (a.slopes) {
-        const float f = (float)d0;
-#pragma unroll
-        for (int r = 0; r < 16; r++)
-          z[r] = __builtin_fmaf(slope, __builtin_fabsf(f + (float)(8 * (r >> 2) + (r & 3))), z[r]);
-      }
-      if (a.table) {
-        if (flat) {
-          const float c = bias[near >= a.reach ? 2 * (a.reach + kBiasPad) : 0];
-#pragma unroll
-          for (int r = 0; r < 16; r++) z[r] += c;
-        } else {
-          const float *at = bias + d0 + a.reach + kBiasPad;
-#pragma unroll
-          for (int r = 0; r < 16; r++) z[r] += at[8 * (r >> 2) + (r & 3)];
-        }
-      }
-    }
+    shape_scores<T, FEAT>(z, by_cap, sc, by, bz);
     float dz[16];
 #pragma unroll
     for (int r = 0; r < 16; r++) dz[r] = exp2_fast(z[r] - lse2) * (dp[r] - delta);
     if (docs || j0 < lo_max || j0 + BK - 1 > hi_min || __ballot(!alive) != 0) {
-      const unsigned e0 = j0 + 4 * h - lo;
+      const unsigned bits = alive ? row_bits(j0, lo, hi, h) : 0;
 #pragma unroll
-      for (int r = 0; r < 16; r++)
-        if (!alive || e0 + (unsigned)(8 * (r >> 2) + (r & 3)) > width) dz[r] = 0.0f;
+      for (int r = 0; r < 16; r++) dz[r] = if_bit(bits, r, dz[r], 0);
       if (docs) {
 #pragma unroll
         for (int g = 0; g < 4; g++) {
@@ -214,7 +200,11 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : 2) void attend_dq_kernel(
       }
     }
     if constexpr (FEAT & kBias) {
-      if (grad_table && mine) {
+      if (grad_table) {
+        if (!mine) {
+#pragma unroll
+          for (int r = 0; r < 16; r++) dz[r] = 0.0f;
+        }
         if (flat) {
           float part = 0.0f;
 #pragma unroll
@@ -224,13 +214,31 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : 2) void attend_dq_kernel(
           else
             below += part;
         } else {
-          // register by register: the 32 queries of a half have 32 distances
-          // to one key, so no two lanes add to one place, and a wave's adds
-          // to its own arrays keep their order
-          typedef __attribute__((address_space(3))) float lfloat;
-          lfloat *const at = (lfloat *)(my_dist + d0 + a.reach + kBiasPad);
+          // Along the tile's diagonals: a row of 64 lanes moves one lane up
+          // for each key and takes up that key's 32 values, so that lane l
+          // ends with the sum at distance j0 - p + 31 - l (p: lane 0's).
+          // A swap with zeros gives both halves' keys as such rows. Two
+          // chains of 16 keys, for the adds' latency; the first, 16 lanes
+          // low, is brought up at the end.
+          float row[2] = {};
 #pragma unroll
-          for (int r = 0; r < 16; r++) __builtin_amdgcn_ds_faddf(at + 8 * (r >> 2) + (r & 3), dz[r], 0, 0, false);
+          for (int g = 0; g < 2; g++) {
+            float up[2][4], dn[2][4];
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+#pragma unroll
+              for (int c = 0; c < 2; c++) halves_apart(dz[4 * (2 * c + g) + e], &up[c][e], &dn[c][e]);
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+#pragma unroll
+              for (int c = 0; c < 2; c++) row[c] = lane_up(row[c]) + up[c][e];
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+#pragma unroll
+              for (int c = 0; c < 2; c++) row[c] = lane_up(row[c]) + dn[c][e];
+          }
+          const float low = __shfl(row[0], lane - 16);
+          my_dist[j0 - p_lo + 31 - lane + a.reach + kBiasPad] += (lane >= 16 ? low : 0.0f) + row[1];
         }
       }
     }
@@ -268,13 +276,13 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : 2) void attend_dq_kernel(
         above += __shfl_xor(above, o);
         below += __shfl_xor(below, o);
       }
-      float *const d = dist + 2 * wave * len;
+      float *const d = dist + wave * len;
       if (lane == 0) d[0] += below, d[len - 1] += above;
       __syncthreads();
       for (int i = tid; i < len; i += THREADS) {
         float v = 0.0f;
 #pragma unroll
-        for (int w = 0; w < 2 * Sh::WAVES; w++) v += dist[w * len + i];
+        for (int w = 0; w < Sh::WAVES; w++) v += dist[w * len + i];
         dist[i] = v;
       }
       __syncthreads();
@@ -330,9 +338,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 || DT == 128 ? 1 : 2) void atte
   query_bounds(a, s, key, &lo, &hi);
   const int k_lo = __builtin_amdgcn_readlane(key, 0), k_hi = __builtin_amdgcn_readlane(key, 31);
   const int lo_min = __builtin_amdgcn_readlane(lo, 0), lo_max = __builtin_amdgcn_readlane(lo, 31);
-  const int hi_min = __builtin_amdgcn_readlane(hi, 0), hi_max = __builtin_amdgcn_readlane(hi, 31);
-  if (hi < lo) lo = 1 << 30, hi = 1 << 30;
-  const unsigned width = hi - lo;
+  const int hi_min = __builtin_amdgcn_readlane(hi, 0);
+  const int hi_max = first + wave * 32 < s.nk ? __builtin_amdgcn_readlane(hi, 31) : INT32_MIN;
   int t_begin, t_end;  // steps of BQ queries
   {
     int l, u, unused;
@@ -372,6 +379,9 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 || DT == 128 ? 1 : 2) void atte
   for (int d = 0; d < ND; d++) dk[d] = v16f{}, dv[d] = v16f{};
 
   QO qt, gt;
+  typename QO::Tags tags;
+  qt.init(a.q.row, a.dim, tid);
+  gt.init(x.g.d_out.row, a.dim, tid);
   float lse = 0.0f, delta = 0.0f;
   int qdoc = 0, buf = 0;
   for (int g = 0; g < x.group; g++) {
@@ -380,18 +390,20 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 || DT == 128 ? 1 : 2) void atte
     const T *const gb = (const T *)x.g.d_out.p + s.q0 * x.g.d_out.row + head * x.g.d_out.head;
     const float *const lse_of = a.lse + (int64_t)head * a.nq + s.q0;
     const float *const delta_of = x.delta + (int64_t)head * a.nq + s.q0;
-    const float slope = (FEAT & kBias) && a.slopes ? -a.slopes[head] * kLog2e : 0.0f;
+    const Bias by{(FEAT & kBias) && a.table ? bias : nullptr,
+                  (FEAT & kBias) && a.slopes ? -a.slopes[head] * bias_unit(a, FEAT & kCap) : 0.0f, a.reach};
     if constexpr (FEAT & kBias) {
       if (a.table) {
         __syncthreads();
-        load_bias<T>(a, head, bias, tid, THREADS);
+        load_bias<T>(a, head, bias_unit(a, FEAT & kCap), bias, tid, THREADS);
       }
     }
     auto fetch = [&](int t) {
-      qt.get(qb, a.q.row, t * BQ, s.nq, a.dim, tid);
-      gt.get(gb, x.g.d_out.row, t * BQ, s.nq, a.dim, tid);
+      const int left = s.nq - t * BQ;
+      qt.get(qb + (int64_t)(t * BQ) * a.q.row, a.q.row, left, tid);
+      gt.get(gb + (int64_t)(t * BQ) * x.g.d_out.row, x.g.d_out.row, left, tid);
       // a row that sees nothing has lse -inf
-      qt.get_tags((const int32_t *)lse_of, t * BQ, s.nq, tid);
+      tags.get((const int32_t *)lse_of + t * BQ, left, tid);
       if (tid < BQ) {
         const int r = min(t * BQ + tid, s.nq - 1);
         lse = lse_of[r];
@@ -413,10 +425,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 || DT == 128 ? 1 : 2) void atte
           qdocs[buf * BQ + tid] = max(qdoc, -1);
         }
         auto keep = [&](int l) { return __builtin_bit_cast(float, l) > -INFINITY; };
-        qt.put(ql, s.nq - t * BQ, a.dim, tid, false, keep);
-#pragma unroll
-        for (int i = 0; i < QO::N; i++) gt.tag[i] = qt.tag[i];
-        gt.put(gl, s.nq - t * BQ, a.dim, tid, false, keep);
+        qt.put(ql, s.nq - t * BQ, a.dim, tid, false, tags, keep);
+        gt.put(gl, s.nq - t * BQ, a.dim, tid, false, tags, keep);
       }
       __syncthreads();
       tn = next(t + 1);
@@ -424,35 +434,16 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 || DT == 128 ? 1 : 2) void atte
       const int p0 = t * BQ + s.shift;  // place of the step's first query
       if (p0 > hi_max || p0 + BQ <= lo_min) continue;
 
-      v16f z = v16f{}, dp = v16f{};
+      v16f z = v16f{}, dp = v16f{}, bz = v16f{};
+      if constexpr (FEAT & kBias) bz = by.template at<-1>(key - p0 - 4 * h, k_lo - p0 - 31, k_hi - p0);
+      if constexpr (FEAT == kBias) z = bz;
 #pragma unroll
       for (int i = 0; i < KS; i++) {
         z = mfma16(QO::rows(ql, 0, i, lane), k[i], z);
         dp = mfma16(QO::rows(gl, 0, i, lane), v[i], dp);
       }
       float by_cap[16];
-      shape_scores<T, FEAT>(z, by_cap, sc);
-      if constexpr (FEAT & kBias) {
-        const int d0 = key - p0 - 4 * h;  // distance at register 0, one less a row
-        if (a.slopes) {
-          const float f = (float)d0;
-#pragma unroll
-          for (int r = 0; r < 16; r++)
-            z[r] = __builtin_fmaf(slope, __builtin_fabsf(f - (float)(8 * (r >> 2) + (r & 3))), z[r]);
-        }
-        if (a.table) {
-          const int near = k_lo - p0 - 31, far = k_hi - p0;
-          if (near >= a.reach || far <= -a.reach) {
-            const float c = bias[near >= a.reach ? 2 * (a.reach + kBiasPad) : 0];
-#pragma unroll
-            for (int r = 0; r < 16; r++) z[r] += c;
-          } else {
-            const float *at = bias + d0 + a.reach + kBiasPad;
-#pragma unroll
-            for (int r = 0; r < 16; r++) z[r] += at[-(8 * (r >> 2) + (r & 3))];
-          }
-        }
-      }
+      shape_scores<T, FEAT>(z, by_cap, sc, by, bz);
       float pr[16];
 #pragma unroll
       for (int g4 = 0; g4 < 4; g4++) {
@@ -461,10 +452,9 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 || DT == 128 ? 1 : 2) void atte
         for (int e = 0; e < 4; e++) pr[4 * g4 + e] = exp2_fast(z[4 * g4 + e] - l[e]);
       }
       if (docs || p0 < lo_max || p0 + BQ - 1 > hi_min) {
-        const unsigned e0 = p0 + 4 * h - lo;
+        const unsigned bits = row_bits(p0, lo, hi, h);
 #pragma unroll
-        for (int r = 0; r < 16; r++)
-          if (e0 + (unsigned)(8 * (r >> 2) + (r & 3)) > width) pr[r] = 0.0f;
+        for (int r = 0; r < 16; r++) pr[r] = if_bit(bits, r, pr[r], 0);
         if (docs) {
 #pragma unroll
           for (int g4 = 0; g4 < 4; g4++) {
@@ -571,7 +561,7 @@ template <class T, int DT, int FEAT>
 bool run_dq(const AttendArgs &x, hipStream_t s) {
   typedef DqShape<T, DT> Sh;
   const int len = (FEAT & kBias) && x.a.table ? attend_bias_len(x.a.reach) : 0;
-  const int shm = Sh::BIAS + 4 * len * (1 + 2 * Sh::WAVES);
+  const int shm = Sh::BIAS + 4 * len * (1 + Sh::WAVES);
   static PerDevice lds;
   if (!lds_granted(lds, (const void *)attend_dq_kernel<T, DT, FEAT>, 160 << 10)) return false;
   attend_dq_kernel<T, DT, FEAT><<<dim3((unsigned)(x.slots * x.a.heads)), Sh::THREADS, shm, s>>>(x);

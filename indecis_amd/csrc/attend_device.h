@@ -15,6 +15,8 @@
 #include <hip/hip_bf16.h>
 #include <hip/hip_fp16.h>
 
+#include <type_traits>
+
 #include "attend.h"
 
 namespace ixh {
@@ -132,6 +134,20 @@ __device__ __forceinline__ float other_half(float v) {
 __device__ __forceinline__ float half_sum(float v) { return v + other_half(v); }
 __device__ __forceinline__ float half_max(float v) { return __builtin_fmaxf(v, other_half(v)); }
 
+// The lower half's values of v with 0 in the upper half, and the upper
+// half's, brought down.
+__device__ __forceinline__ void halves_apart(float v, float *low, float *high) {
+  typedef unsigned u2 __attribute__((ext_vector_type(2)));
+  const u2 r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, v), 0u, false, false);
+  const unsigned a = r[0], b = r[1];  // a bit cast of r[1] itself reads r[0]
+  *low = __builtin_bit_cast(float, a);
+  *high = __builtin_bit_cast(float, b);
+}
+// Every lane's value from the lane below, lane 0's 0 (wave_shr:1).
+__device__ __forceinline__ float lane_up(float v) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x138, 0xf, 0xf, true));
+}
+
 // ---- tiles of rows in LDS ---------------------------------------------------
 // R rows of DT values, 16-byte pieces; piece c of row r stands at c ^ (r & 7),
 // so that the 16 rows a quarter-wave reads of one column of pieces, and the 8
@@ -144,35 +160,47 @@ struct Tile {
   static constexpr int BYTES = R * RB;
   static constexpr int N = R * CH / THREADS;       // pieces a thread
   static_assert(N * THREADS == R * CH && CH >= 8, "");
+  static constexpr int STEP = THREADS / CH;        // rows between a thread's pieces
+  static_assert(THREADS % CH == 0, "");
   i4 part[N];
-  int tag[N];
+  unsigned off;  // of the thread's first piece, in bytes from the tile's first row
 
-  // Starts the loads of rows r0.. of the sequence (n rows in all, from base):
-  // a row past the last and a piece past `dim` are read where there is one
-  // and dropped in put().
-  __device__ __forceinline__ void get(const T *base, int64_t stride, int r0, int n, int dim, int tid) {
+  // A piece past `dim` is read as the row's first and dropped in put().
+  __device__ __forceinline__ void init(int64_t stride, int dim, int tid) {
+    const int r = tid / CH, c = tid % CH;
+    off = (unsigned)(r * stride * sizeof(T)) + (c * EPC < dim ? 16 * c : 0);
+  }
+  // Starts the loads of the rows at `first`, `left` of which there are: a row
+  // past them is read as the last and dropped in put().
+  __device__ __forceinline__ void get(const T *first, int64_t stride, int left, int tid) {
+    if (left >= R) {
 #pragma unroll
-    for (int i = 0; i < N; i++) {
-      const int at = tid + i * THREADS, r = at / CH, c = at % CH;
-      const int row = min(r0 + r, n - 1);
-      const int col = c * EPC < dim ? c * EPC : 0;
-      part[i] = *(const i4 *)(base + row * stride + col);
+      for (int i = 0; i < N; i++) part[i] = *(const i4 *)((const char *)(first + i * STEP * stride) + off);
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; i++) {
+        const int past = max(tid / CH + i * STEP - (left - 1), 0);
+        part[i] = *(const i4 *)((const char *)(first + (i * STEP - past) * stride) + off);
+      }
     }
   }
   // Starts the loads of those rows' tags, by which put() may drop them too.
-  __device__ __forceinline__ void get_tags(const int32_t *base, int r0, int n, int tid) {
+  struct Tags {
+    int v[N];
+    __device__ __forceinline__ void get(const int32_t *first, int left, int tid) {
 #pragma unroll
-    for (int i = 0; i < N; i++) tag[i] = base[min(r0 + (tid + i * THREADS) / CH, n - 1)];
-  }
-  // Writes them; what is past `rows` rows or `dim` columns, and rows whose
+      for (int i = 0; i < N; i++) v[i] = first[min(tid / CH + i * STEP, left - 1)];
+    }
+  };
+  // Writes them; what is past `left` rows or `dim` columns, and rows whose
   // tag keep() refuses, as 0. all: nothing is.
   template <class Keep>
-  __device__ __forceinline__ void put(char *lds, int rows, int dim, int tid, bool all, Keep keep) {
+  __device__ __forceinline__ void put(char *lds, int left, int dim, int tid, bool all, const Tags &tags, Keep keep) {
 #pragma unroll
     for (int i = 0; i < N; i++) {
-      const int at = tid + i * THREADS, r = at / CH, c = at % CH;
+      const int r = tid / CH + i * STEP, c = tid % CH;
       i4 v = part[i];
-      if (!all && !(c * EPC < dim && r < rows && keep(tag[i]))) v = i4{0, 0, 0, 0};
+      if (!all && !(c * EPC < dim && r < left && keep(tags.v[i]))) v = i4{0, 0, 0, 0};
       *(i4 *)(lds + r * RB + ((c ^ (r & 7)) << 4)) = v;
     }
   }
@@ -361,33 +389,90 @@ struct Score {
   }
 };
 
-// tanh(x) = 1 - 2u, u = 1 / (1 + e^2x), with the hardware's exponential and
-// reciprocal: off by about 1e-7 of 1, which next to a 16-bit result is
-// nothing; float32 takes the library's tanh. *u serves the derivative,
-// 1 - tanh^2 = 4 u (1 - u).
+// c2 tanh(s c1): tanh(x) = 1 - 2u, u = 1 / (1 + e^2x), with the hardware's
+// exponential and reciprocal: off by about 1e-7 of 1, which next to a 16-bit
+// result is nothing; float32 takes the library's tanh. *u serves the
+// derivative, 1 - tanh^2 = 4 u (1 - u).
 template <class T>
-__device__ __forceinline__ float tanh_of(float x, float *u) {
+__device__ __forceinline__ float capped(const Score &sc, float s, float *u) {
   if constexpr (sizeof(T) == 4) {
-    const float t = tanhf(x);
+    const float t = tanhf(s * sc.c1);
     *u = 0.5f - 0.5f * t;
-    return t;
+    return sc.c2 * t;
   } else {
-    const float e = exp2_fast(x * (2 * kLog2e));
+    const float e = exp2_fast(s * (sc.c1 * (2 * kLog2e)));
     *u = __builtin_amdgcn_rcpf(1.0f + e);
-    return __builtin_fmaf(-2.0f, *u, 1.0f);
+    return __builtin_fmaf(*u, -2.0f * sc.c2, sc.c2);
   }
 }
 
-// The bias of one head: slope (base 2) and the table by distance, copied to
-// LDS in base 2 with its ends drawn out by kBiasPad.
+// The bias starts the first product's sum, in units of q.k (bias / scale), so
+// that it costs no operation of its own; under a cap it is added to z, in
+// base 2.
+__device__ __forceinline__ float bias_unit(const ixh_attend_args &a, bool cap) { return cap ? kLog2e : 1.0f / a.scale; }
+
+// One head's bias table by distance, copied to LDS with its ends drawn out
+// by kBiasPad.
 template <class T>
-__device__ __forceinline__ void load_bias(const ixh_attend_args &a, int head, float *lds, int tid, int threads) {
+__device__ __forceinline__ void load_bias(const ixh_attend_args &a, int head, float unit, float *lds, int tid,
+                                          int threads) {
   const int len = attend_bias_len(a.reach);
   for (int i = tid; i < len; i += threads) {
     const int d = min(max(i - a.reach - kBiasPad, -a.reach), a.reach);
     const int b = a.buckets[d + a.reach];
-    lds[i] = b >= 0 && b < a.n_buckets ? (float)((const T *)a.table)[(int64_t)b * a.heads + head] * kLog2e : 0.0f;
+    lds[i] = b >= 0 && b < a.n_buckets ? (float)((const T *)a.table)[(int64_t)b * a.heads + head] * unit : 0.0f;
   }
+}
+
+// One head's bias of a lane's 16 scores of a 32x32 tile. d0: the distance at
+// register 0, which grows by `sign` a row; near..far: the tile's distances.
+struct Bias {
+  const float *tab;  // nullptr: no table
+  float slope;       // 0: none
+  int reach;
+  template <int SIGN>
+  __device__ __forceinline__ v16f at(int d0, int near, int far) const {
+    v16f z{};
+    if (tab) {
+      if (near >= reach || far <= -reach) {
+        const float c = tab[near >= reach ? 2 * (reach + kBiasPad) : 0];
+#pragma unroll
+        for (int r = 0; r < 16; r++) z[r] = c;
+      } else {
+        const float *p = tab + d0 + reach + kBiasPad;
+#pragma unroll
+        for (int r = 0; r < 16; r++) z[r] = p[SIGN * (8 * (r >> 2) + (r & 3))];
+      }
+    }
+    if (slope != 0.0f) {
+      const float f = (float)d0;
+#pragma unroll
+      for (int r = 0; r < 16; r++)
+        z[r] = __builtin_fmaf(slope, __builtin_fabsf(f + (float)(SIGN * (8 * (r >> 2) + (r & 3)))), z[r]);
+    }
+    return z;
+  }
+};
+
+// ---- masks ------------------------------------------------------------------
+// The lane's rows of a 32-row tile from j0 on that lie in lo..hi, a bit each,
+// bit 8 (r / 4) + r % 4 its register r's.
+__device__ __forceinline__ unsigned row_bits(int j0, int lo, int hi, int h) {
+  const int l = min(max(lo - j0, 0), 32), u = min(max(hi + 1 - j0, 0), 32);
+  const unsigned below = (unsigned)((1ull << l) - 1), upto = (unsigned)((1ull << u) - 1);
+  return (upto & ~below) >> (4 * h);
+}
+// v where the bit of register r is set, else `other`.
+__device__ __forceinline__ float if_bit(unsigned bits, int r, float v, unsigned other) {
+  const unsigned m = (unsigned)__builtin_amdgcn_sbfe((int)bits, 8 * (r >> 2) + (r & 3), 1);
+  return __builtin_bit_cast(float, (__builtin_bit_cast(unsigned, v) & m) | (other & ~m));
+}
+constexpr unsigned kMinusInf = 0xff800000u;
+
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(d) : "v"(a), "v"(b), "v"(c));
+  return d;
 }
 
 }  // namespace ixh

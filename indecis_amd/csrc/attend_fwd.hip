@@ -24,7 +24,8 @@ struct FwdShape {
 };
 
 template <class T, int DT, int WAVES, int FEAT>
-__global__ __launch_bounds__(64 * WAVES, 2) void attend_fwd_kernel(AttendArgs x) {
+__global__ __launch_bounds__(64 * WAVES, sizeof(T) * DT == 128 ? 3 : sizeof(T) * DT == 512 && WAVES == 1 ? 1 : 2)
+void attend_fwd_kernel(AttendArgs x) {
   typedef FwdShape<T, DT, WAVES> Sh;
   typedef typename Sh::KV KV;
   typedef typename Kind<T>::frag Frag;
@@ -51,16 +52,16 @@ __global__ __launch_bounds__(64 * WAVES, 2) void attend_fwd_kernel(AttendArgs x)
   // the lane's query: row, head, place; rows past the last repeat it
   const int64_t r = min(blk * ROWS + wave * 32 + (lane & 31), rows - 1);
   const bool mine = blk * ROWS + wave * 32 + (lane & 31) < rows;
-  const int tok = pack > 1 ? (int)(r / pack) : (int)r, sub = pack > 1 ? (int)(r - (int64_t)tok * pack) : 0;
+  const int tok = pack > 1 ? (int)((unsigned)r / (unsigned)pack) : (int)r, sub = pack > 1 ? (int)(r - (int64_t)tok * pack) : 0;
   const int head = pack > 1 ? hb * pack + sub : hb;
   const int p = tok + s.shift;
   int lo, hi;
   key_bounds(a, s, p, &lo, &hi);
   const int p_lo = __builtin_amdgcn_readlane(p, 0), p_hi = __builtin_amdgcn_readlane(p, 31);
   const int lo_min = __builtin_amdgcn_readlane(lo, 0), lo_max = __builtin_amdgcn_readlane(lo, 31);
-  const int hi_min = __builtin_amdgcn_readlane(hi, 0), hi_max = __builtin_amdgcn_readlane(hi, 31);
-  if (hi < lo) lo = 1 << 30, hi = 1 << 30;  // sees nothing: no key is there
-  const unsigned width = hi - lo;
+  const int hi_min = __builtin_amdgcn_readlane(hi, 0);
+  // a wave past the last row has nothing to see
+  const int hi_max = blk * ROWS + wave * 32 < rows ? __builtin_amdgcn_readlane(hi, 31) : -1;
 
   // the workgroup's steps of keys
   int t_begin, t_end;
@@ -89,7 +90,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void attend_fwd_kernel(AttendArgs x)
   if constexpr (FEAT & kBias) {
     if (a.table)
       for (int i = 0; i < pack; i++)
-        load_bias<T>(a, pack > 1 ? hb * pack + i : hb, bias + i * attend_bias_len(a.reach), tid, THREADS);
+        load_bias<T>(a, pack > 1 ? hb * pack + i : hb, bias_unit(a, FEAT & kCap), bias + i * attend_bias_len(a.reach), tid, THREADS);
   }
   if (a.q_docs || (FEAT & kBias)) __syncthreads();
 
@@ -105,8 +106,8 @@ __global__ __launch_bounds__(64 * WAVES, 2) void attend_fwd_kernel(AttendArgs x)
   const T *const kb = (const T *)a.k.p + s.k0 * a.k.row + kvh * a.k.head;
   const T *const vb = (const T *)a.v.p + s.k0 * a.v.row + kvh * a.v.head;
   const Score sc(a, FEAT & kCap);
-  const float slope = (FEAT & kBias) && a.slopes ? -a.slopes[head] * kLog2e : 0.0f;
-  const float *const tab = bias + sub * attend_bias_len(a.reach);
+  const Bias by{(FEAT & kBias) && a.table ? bias + sub * attend_bias_len(a.reach) : nullptr,
+                (FEAT & kBias) && a.slopes ? -a.slopes[head] * bias_unit(a, FEAT & kCap) : 0.0f, a.reach};
 
   v16f acc[ND];
 #pragma unroll
@@ -114,13 +115,99 @@ __global__ __launch_bounds__(64 * WAVES, 2) void attend_fwd_kernel(AttendArgs x)
   float m = -INFINITY, ref = 0.0f, sum = 0.0f;  // maximum so far; what scores are taken against
 
   KV kt, vt;
+  typename KV::Tags tags;
+  kt.init(a.k.row, a.dim, tid);
+  vt.init(a.v.row, a.dim, tid);
   int kdoc = 0;
   auto fetch = [&](int t) {
-    kt.get(kb, a.k.row, t * BK, s.nk, a.dim, tid);
-    vt.get(vb, a.v.row, t * BK, s.nk, a.dim, tid);
+    const int left = s.nk - t * BK;
+    kt.get(kb + (int64_t)(t * BK) * a.k.row, a.k.row, left, tid);
+    vt.get(vb + (int64_t)(t * BK) * a.v.row, a.v.row, left, tid);
     if (a.q_docs) {
-      kt.get_tags(a.k_docs + s.k0, t * BK, s.nk, tid);
-      if (tid < BK) kdoc = a.k_docs[s.k0 + min(t * BK + tid, s.nk - 1)];
+      tags.get(a.k_docs + s.k0 + t * BK, left, tid);
+      if (tid < BK) kdoc = a.k_docs[s.k0 + t * BK + min(tid, left - 1)];
+    }
+  };
+
+  // N 32-key tiles from key j0 of the sequence, rows r0 of the step in LDS:
+  // scores, running maximum and sum, and their part of the output.
+  auto tiles = [&](auto count, int j0, int r0, const char *kl, const char *vl, const int *kd) {
+    constexpr int N = count.value;
+    v16f z[N];
+#pragma unroll
+    for (int u = 0; u < N; u++) {
+      z[u] = v16f{};
+      if constexpr (FEAT == kBias) z[u] = by.template at<1>(j0 + 32 * u + 4 * h - p, j0 + 32 * u - p_hi, j0 + 32 * u + 31 - p_lo);
+#pragma unroll
+      for (int i = 0; i < KS; i++) z[u] = mfma16(KV::rows(kl, r0 + 32 * u, i, lane), q[i], z[u]);
+    }
+    const bool masked = kd || j0 < lo_max || j0 + 32 * N - 1 > hi_min;
+    if constexpr (FEAT & kCap) {
+#pragma unroll
+      for (int u = 0; u < N; u++) {
+#pragma unroll
+        for (int r = 0; r < 16; r++) {
+          float unused;
+          z[u][r] = capped<T>(sc, z[u][r], &unused);
+        }
+        if constexpr (FEAT & kBias)
+          z[u] += by.template at<1>(j0 + 32 * u + 4 * h - p, j0 + 32 * u - p_hi, j0 + 32 * u + 31 - p_lo);
+      }
+    }
+    if (masked) {
+#pragma unroll
+      for (int u = 0; u < N; u++) {
+        const unsigned bits = row_bits(j0 + 32 * u, lo, hi, h);
+#pragma unroll
+        for (int r = 0; r < 16; r++) z[u][r] = if_bit(bits, r, z[u][r], kMinusInf);
+        if (kd) {
+#pragma unroll
+          for (int g = 0; g < 4; g++) {
+            const i4 d = *(const i4 *)(kd + r0 + 32 * u + 8 * g + 4 * h);
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+              if (d[e] != doc) z[u][4 * g + e] = -INFINITY;
+          }
+        }
+      }
+    }
+    float top = z[0][0];
+#pragma unroll
+    for (int u = 0; u < N; u++)
+#pragma unroll
+      for (int r = 0; r < 16; r += 2) top = max3(z[u][r], z[u][r + 1], top);
+    top = half_max(top);
+    if constexpr (!(FEAT & kCap)) top *= sc.c1;
+    // the sums keep an old maximum until it is 2^8 short: they stay far
+    // inside every type's range, and few steps rescale
+    if (__ballot(top > m + 8.0f)) {
+      const float next_m = __builtin_fmaxf(m, top);
+      const float f = m == -INFINITY ? 0.0f : exp2_fast(m - next_m);
+      m = next_m;
+      ref = m == -INFINITY ? 0.0f : m;
+      sum *= f;
+#pragma unroll
+      for (int d = 0; d < ND; d++)
+#pragma unroll
+        for (int r = 0; r < 16; r++) acc[d][r] *= f;
+    }
+#pragma unroll
+    for (int u = 0; u < N; u++) {
+      float part = 0.0f, pr[16];
+#pragma unroll
+      for (int r = 0; r < 16; r++) {
+        pr[r] = exp2_fast((FEAT & kCap) ? z[u][r] - ref : __builtin_fmaf(z[u][r], sc.c1, -ref));
+        part += pr[r];
+      }
+      sum += part;
+      // the probabilities are rounded to the rows' type here, as V is: the
+      // product's sum stays in 32 bits
+#pragma unroll
+      for (int v = 0; v < 2; v++) {
+        const Frag pf = pack8<Frag>(pr + 8 * v);
+#pragma unroll
+        for (int d = 0; d < ND; d++) acc[d] = mfma16(KV::cols(vl, r0 + 32 * u + 16 * v, d, lane), pf, acc[d]);
+      }
     }
   };
 
@@ -135,117 +222,29 @@ __global__ __launch_bounds__(64 * WAVES, 2) void attend_fwd_kernel(AttendArgs x)
       const bool all = a.dim == DT && t * BK + BK <= s.nk && !docs;
       auto keep = [&](int d) { return !docs || d >= 0; };
       if (docs && tid < BK) kdocs[buf * BK + tid] = kdoc < 0 ? -2 : kdoc;
-      kt.put(kl, s.nk - t * BK, a.dim, tid, all, keep);
-#pragma unroll
-      for (int i = 0; i < KV::N; i++) vt.tag[i] = kt.tag[i];
-      vt.put(vl, s.nk - t * BK, a.dim, tid, all, keep);
+      kt.put(kl, s.nk - t * BK, a.dim, tid, all, tags, keep);
+      vt.put(vl, s.nk - t * BK, a.dim, tid, all, tags, keep);
     }
     __syncthreads();
     const int tn = next(t + 1);
     if (tn < t_end) fetch(tn);
 
     const int j0 = t * BK;
-    if (j0 <= hi_max && j0 + BK > lo_min) {
-      v16f z[NS];
-#pragma unroll
-      for (int u = 0; u < NS; u++) {
-        z[u] = v16f{};
-#pragma unroll
-        for (int i = 0; i < KS; i++) z[u] = mfma16(KV::rows(kl, 32 * u, i, lane), q[i], z[u]);
-      }
-      const bool masked = docs || j0 < lo_max || j0 + BK - 1 > hi_min;
-      if constexpr (FEAT != 0) {
-#pragma unroll
-        for (int u = 0; u < NS; u++) {
-          const int d0 = j0 + 32 * u + 4 * h - p;  // distance of register 0
-          if constexpr (FEAT & kCap) {
-#pragma unroll
-            for (int r = 0; r < 16; r++) {
-              float unused;
-              z[u][r] = sc.c2 * tanh_of<T>(z[u][r] * sc.c1, &unused);
-            }
-          } else {
-#pragma unroll
-            for (int r = 0; r < 16; r++) z[u][r] *= sc.c1;
-          }
-          if constexpr (FEAT & kBias) {
-            if (a.slopes) {
-              const float f = (float)d0;
-#pragma unroll
-              for (int r = 0; r < 16; r++)
-                z[u][r] = __builtin_fmaf(slope, __builtin_fabsf(f + (float)(8 * (r >> 2) + (r & 3))), z[u][r]);
-            }
-            if (a.table) {
-              const int near = j0 + 32 * u - p_hi, far = j0 + 32 * u + 31 - p_lo;
-              if (near >= a.reach || far <= -a.reach) {
-                const float c = tab[near >= a.reach ? 2 * (a.reach + kBiasPad) : 0];
-#pragma unroll
-                for (int r = 0; r < 16; r++) z[u][r] += c;
-              } else {
-                const float *at = tab + d0 + a.reach + kBiasPad;
-#pragma unroll
-                for (int r = 0; r < 16; r++) z[u][r] += at[8 * (r >> 2) + (r & 3)];
-              }
-            }
-          }
-        }
-      }
-      if (masked) {
-#pragma unroll
-        for (int u = 0; u < NS; u++) {
-          const unsigned e0 = j0 + 32 * u + 4 * h - lo;
-#pragma unroll
-          for (int r = 0; r < 16; r++)
-            if (e0 + (unsigned)(8 * (r >> 2) + (r & 3)) > width) z[u][r] = -INFINITY;
-          if (docs) {
-#pragma unroll
-            for (int g = 0; g < 4; g++) {
-              const i4 d = *(const i4 *)(kdocs + buf * BK + 32 * u + 8 * g + 4 * h);
-#pragma unroll
-              for (int e = 0; e < 4; e++)
-                if (d[e] != doc) z[u][4 * g + e] = -INFINITY;
-            }
-          }
-        }
-      }
-      float top = z[0][0];
-#pragma unroll
-      for (int u = 0; u < NS; u++)
-#pragma unroll
-        for (int r = 0; r < 16; r++) top = __builtin_fmaxf(top, z[u][r]);
-      top = half_max(top);
-      if constexpr (FEAT == 0) top *= sc.c1;
-      // the sums keep an old maximum until it is 2^8 short: they stay far
-      // inside every type's range, and few steps rescale
-      if (__ballot(top > m + 8.0f)) {
-        const float next_m = __builtin_fmaxf(m, top);
-        const float f = m == -INFINITY ? 0.0f : exp2_fast(m - next_m);
-        m = next_m;
-        ref = m == -INFINITY ? 0.0f : m;
-        sum *= f;
-#pragma unroll
-        for (int d = 0; d < ND; d++)
-#pragma unroll
-          for (int r = 0; r < 16; r++) acc[d][r] *= f;
-      }
-#pragma unroll
-      for (int u = 0; u < NS; u++) {
-        float part = 0.0f, pr[16];
-#pragma unroll
-        for (int r = 0; r < 16; r++) {
-          pr[r] = exp2_fast(FEAT == 0 ? __builtin_fmaf(z[u][r], sc.c1, -ref) : z[u][r] - ref);
-          part += pr[r];
-        }
-        sum += part;
-        // the probabilities are rounded to the rows' type here, as V is: the
-        // product's sum stays in 32 bits
-#pragma unroll
-        for (int v = 0; v < 2; v++) {
-          const Frag pf = pack8<Frag>(pr + 8 * v);
-#pragma unroll
-          for (int d = 0; d < ND; d++) acc[d] = mfma16(KV::cols(vl, 32 * u + 16 * v, d, lane), pf, acc[d]);
-        }
-      }
+    const int *const kd = docs ? kdocs + buf * BK : nullptr;
+    auto live_at = [&](int j) { return j <= hi_max && j + 31 >= lo_min; };
+    if constexpr (NS == 1) {
+      if (live_at(j0)) tiles(std::integral_constant<int, 1>(), j0, 0, kl, vl, kd);
+    } else if constexpr (DT > 64) {
+      // one at a time: two tiles' scores beside 64 sums spill
+#pragma unroll 1
+      for (int u = 0; u < 2; u++)
+        if (live_at(j0 + 32 * u)) tiles(std::integral_constant<int, 1>(), j0 + 32 * u, 32 * u, kl, vl, kd);
+    } else {
+      const bool first = live_at(j0), last = live_at(j0 + 32);
+      if (first && last)
+        tiles(std::integral_constant<int, 2>(), j0, 0, kl, vl, kd);
+      else if (first || last)
+        tiles(std::integral_constant<int, 1>(), last ? j0 + 32 : j0, last ? 32 : 0, kl, vl, kd);
     }
     buf ^= 1;
     t = tn;
