@@ -14,6 +14,7 @@ columns of one projection): strides and pointers are multiples of 16 bytes,
 the values of a head stand side by side.
 """
 import ctypes as C
+import struct
 
 import numpy as np
 import torch
@@ -22,92 +23,107 @@ from . import _lib
 
 _TYPES = {torch.float32: _lib.TYPE_F32, torch.bfloat16: _lib.TYPE_BF16, torch.float16: _lib.TYPE_F16}
 
+# The library's argument structs, packed in one go: a call of the smallest
+# size is as long as its host side.
+_ATTEND = struct.Struct("@7i" + 4 * "Pqq" + "2P2f3P2i2PiPi2Pq")
+_GRADS = struct.Struct("@" + 4 * "Pqq" + "P")
+_NORM_ROPE = struct.Struct("@5i" + 4 * "Pqq" + "idi4P3iP" + "Pq")
+_NORM_ROPE_GRADS = struct.Struct("@" + 4 * "Pqq" + "2P")
+for _s, _c in ((_ATTEND, _lib.IxhAttendArgs), (_GRADS, _lib.IxhAttendGrads), (_NORM_ROPE, _lib.IxhNormRopeArgs),
+               (_NORM_ROPE_GRADS, _lib.IxhNormRopeGrads)):
+    assert _s.size == C.sizeof(_c)
+
 
 def _need(ok, op, what):
     if not ok:
         raise ValueError(f"linalg: {op}: {what}")
 
 
-def _rows(op, name, t, like=None):
-    """Checks rows of heads; `like`: a tensor with the same type and GPU."""
-    _need(t.dim() == 3, op, f"{name} is not [rows][heads][dim]")
-    _need(t.dtype in _TYPES, op, f"{name} of type {t.dtype}")
-    _need(t.is_cuda, op, f"{name} is not on a GPU")
-    _need(t.shape[2] == 0 or t.stride(2) == 1, op, f"{name}: the values of a head do not stand side by side")
-    if like is not None:
-        _need(t.dtype == like.dtype and t.device == like.device, op, f"{name} has another type or GPU")
-
-
-def _heads(t):
+def _heads(op, name, t, like=None, shape=None):
+    """(address, row stride, head stride) of rows of heads; `like`: a tensor
+    with the same type and GPU."""
+    size, strides = t.shape, t.stride()
+    if (len(size) != 3 or not t.is_cuda or (strides[2] != 1 and size[2] > 0) or (like is None and t.dtype not in _TYPES)
+            or (like is not None and (t.dtype is not like.dtype or t.get_device() != like.get_device()))
+            or (shape is not None and size != shape)):
+        _need(len(size) == 3, op, f"{name} is not [rows][heads][dim]")
+        _need(t.dtype in _TYPES, op, f"{name} of type {t.dtype}")
+        _need(t.is_cuda, op, f"{name} is not on a GPU")
+        _need(strides[2] == 1 or size[2] == 0, op, f"{name}: the values of a head do not stand side by side")
+        _need(like is None or (t.dtype is like.dtype and t.get_device() == like.get_device()), op,
+              f"{name} has another type or GPU")
+        _need(False, op, f"{name} is not of shape {tuple(shape)}")
+    n, h, d = size
     # the stride along one row or one head says nothing
-    n, h, d = t.shape
-    head = t.stride(1) if h > 1 else d
-    return _lib.IxhHeads(t.data_ptr(), t.stride(0) if n > 1 else h * d, head)
+    return t.data_ptr(), strides[0] if n > 1 else h * d, strides[1] if h > 1 else d
 
 
 def _plain(op, name, t, like, dtype, shape):
-    """The address of a contiguous array on like's GPU, or None."""
+    """The address of a contiguous array on like's GPU; 0 for None."""
     if t is None:
-        return None
-    _need(t.dtype == dtype and tuple(t.shape) == shape, op, f"{name} is not {dtype} of shape {shape}")
-    _need(t.device == like.device and t.is_contiguous(), op, f"{name} is not contiguous on the rows' GPU")
+        return 0
+    if t.dtype is not dtype or t.shape != shape or t.get_device() != like.get_device() or not t.is_contiguous():
+        _need(t.dtype is dtype and t.shape == shape, op, f"{name} is not {dtype} of shape {tuple(shape)}")
+        _need(False, op, f"{name} is not contiguous on the rows' GPU")
     return t.data_ptr()
 
 
-def _out(op, name, t, like, shape):
+def _out(op, name, t, like):
+    """An output of like's shape, and its place."""
     if t is None:
-        return torch.empty(shape, dtype=like.dtype, device=like.device)
-    _rows(op, name, t, like)
-    _need(tuple(t.shape) == shape, op, f"{name} is not of shape {shape}")
-    return t
+        t = torch.empty(like.shape, dtype=like.dtype, device=like.device)
+    return t, _heads(op, name, t, like, like.shape)
 
 
-def _stream(t):
-    return torch.cuda.current_stream(t.device).cuda_stream
+def _call(f, like, *args):
+    device = like.get_device()
+    _lib.check(f(device, *args, torch.cuda.current_stream(device).cuda_stream))
 
 
-def _space(t, n):
-    return torch.empty(n, dtype=torch.uint8, device=t.device) if n else None
+def _space(like, n):
+    return torch.empty(n, dtype=torch.uint8, device=like.device) if n else None
 
 
 def _attend_args(op, q, k, v, offs, k_offs, scale, cap, slopes, table, buckets, docs, k_docs, causal, prefix, window):
-    _rows(op, "q", q)
-    _rows(op, "k", k, q)
-    _rows(op, "v", v, q)
+    """The values of ixh_attend_args before and after o, up to lse."""
+    qh, kh, vh = _heads(op, "q", q), _heads(op, "k", k, q), _heads(op, "v", v, q)
     nq, heads, dim = q.shape
-    nk, kv_heads, _ = k.shape
-    _need(k.shape == v.shape and k.shape[2] == dim, op, "q, k and v do not fit together")
+    nk, kv_heads, k_dim = k.shape
+    _need(k.shape == v.shape and k_dim == dim, op, "q, k and v do not fit together")
     _need(offs.dim() == 1 and len(offs) >= 1, op, "offs is not [sequences + 1]")
     B = len(offs) - 1
-    a = _lib.IxhAttendArgs()
-    a.type, a.B, a.nq, a.nk, a.heads, a.kv_heads, a.dim = _TYPES[q.dtype], B, nq, nk, heads, kv_heads, dim
-    a.q, a.k, a.v = _heads(q), _heads(k), _heads(v)
-    a.q_offs = _plain(op, "offs", offs, q, torch.int32, (B + 1,))
-    a.k_offs = _plain(op, "k_offs", k_offs, q, torch.int32, (B + 1,))
-    a.scale = dim ** -0.5 if scale is None else scale
-    a.cap = cap
-    a.slopes = _plain(op, "slopes", slopes, q, torch.float32, (heads,))
+    n_buckets = reach = 0
     if table is not None:
         _need(table.dim() == 2 and buckets is not None and buckets.dim() == 1 and len(buckets) % 2 == 1, op,
               "a table [buckets][heads] needs the buckets of an odd number of distances")
-        a.n_buckets, a.reach = len(table), len(buckets) // 2
-        a.table = _plain(op, "table", table, q, q.dtype, (len(table), heads))
-        a.buckets = _plain(op, "buckets", buckets, q, torch.int32, (len(buckets),))
-    a.q_docs = _plain(op, "docs", docs, q, torch.int32, (nq,))
-    a.k_docs = _plain(op, "k_docs", k_docs, q, torch.int32, (nk,))
-    a.causal = 1 if causal else 0
-    a.prefix = _plain(op, "prefix", prefix, q, torch.int32, (B,))
-    a.window = -1 if window is None else window
-    return a
+        n_buckets, reach = len(table), len(buckets) // 2
+    i32 = torch.int32
+    return (_TYPES[q.dtype], B, nq, nk, heads, kv_heads, dim, *qh, *kh, *vh), (
+        _plain(op, "offs", offs, q, i32, (B + 1,)),
+        _plain(op, "k_offs", k_offs, q, i32, (B + 1,)),
+        dim ** -0.5 if scale is None else scale, cap,
+        _plain(op, "slopes", slopes, q, torch.float32, (heads,)),
+        _plain(op, "table", table, q, q.dtype, (n_buckets, heads)),
+        _plain(op, "buckets", buckets, q, i32, (2 * reach + 1,)) if table is not None else 0,
+        n_buckets, reach,
+        _plain(op, "docs", docs, q, i32, (nq,)),
+        _plain(op, "k_docs", k_docs, q, i32, (nk,)),
+        1 if causal else 0,
+        _plain(op, "prefix", prefix, q, i32, (B,)),
+        -1 if window is None else window)
 
 
-def _with_space(a, q, backward):
+def _with_space(args, q, backward):
+    """The packed arguments with their workspace, and the workspace: held
+    until the call has queued its work."""
     n = C.c_int64()
-    _lib.check(_lib.lib().ixh_attend_workspace(C.byref(a), backward, C.byref(n)))
+    L = _lib.lib()
+    packed = _ATTEND.pack(*args, 0, 0)
+    _lib.check(L.ixh_attend_workspace(packed, backward, C.byref(n)))
+    if n.value == 0:
+        return packed, None
     space = _space(q, n.value)
-    if space is not None:
-        a.workspace, a.workspace_bytes = space.data_ptr(), n.value
-    return space
+    return _ATTEND.pack(*args, space.data_ptr(), n.value), space
 
 
 def attend(q, k, v, offs, k_offs=None, *, scale=None, cap=0.0, slopes=None, table=None, buckets=None, docs=None,
@@ -127,13 +143,12 @@ def attend(q, k, v, offs, k_offs=None, *, scale=None, cap=0.0, slopes=None, tabl
     far off. A query that sees nothing gets 0 (and -inf). Rows outside the
     sequences are left as they are."""
     op = "Attend"
-    a = _attend_args(op, q, k, v, offs, k_offs, scale, cap, slopes, table, buckets, docs, k_docs, causal, prefix, window)
-    out = _out(op, "out", out, q, tuple(q.shape))
-    lse = torch.empty((a.heads, a.nq), dtype=torch.float32, device=q.device) if want_lse else None
-    a.o = _heads(out)
-    a.lse = lse.data_ptr() if want_lse else None
-    space = _with_space(a, q, 0)  # held until the call has queued its work
-    _lib.check(_lib.lib().ixh_attend(q.device.index, C.byref(a), _stream(q)))
+    before, after = _attend_args(op, q, k, v, offs, k_offs, scale, cap, slopes, table, buckets, docs, k_docs, causal,
+                                 prefix, window)
+    out, place = _out(op, "out", out, q)
+    lse = torch.empty((q.shape[1], q.shape[0]), dtype=torch.float32, device=q.device) if want_lse else None
+    args, space = _with_space((*before, *place, *after, lse.data_ptr() if want_lse else 0), q, 0)
+    _call(_lib.lib().ixh_attend, q, args)
     return (out, lse) if want_lse else out
 
 
@@ -144,20 +159,17 @@ def attend_backward(d_out, q, k, v, out, lse, offs, k_offs=None, *, scale=None, 
     from its output and lse; dtable [buckets][heads] of the table's type, None
     without a table."""
     op = "AttendBackward"
-    a = _attend_args(op, q, k, v, offs, k_offs, scale, cap, slopes, table, buckets, docs, k_docs, causal, prefix, window)
-    for name, t in (("d_out", d_out), ("out", out)):
-        _rows(op, name, t, q)
-        _need(t.shape == q.shape, op, f"{name} is not of q's shape")
-    dq = _out(op, "dq", dq, q, tuple(q.shape))
-    dk = _out(op, "dk", dk, q, tuple(k.shape))
-    dv = _out(op, "dv", dv, q, tuple(v.shape))
-    dtable = torch.empty_like(table) if table is not None else None
+    before, after = _attend_args(op, q, k, v, offs, k_offs, scale, cap, slopes, table, buckets, docs, k_docs, causal,
+                                 prefix, window)
     _need(lse is not None, op, "lse is missing")
-    a.o, a.lse = _heads(out), _plain(op, "lse", lse, q, torch.float32, (a.heads, a.nq))
-    g = _lib.IxhAttendGrads(_heads(d_out), _heads(dq), _heads(dk), _heads(dv),
-                            None if dtable is None else dtable.data_ptr())
-    space = _with_space(a, q, 1)
-    _lib.check(_lib.lib().ixh_attend_backward(q.device.index, C.byref(a), C.byref(g), _stream(q)))
+    lse_at = _plain(op, "lse", lse, q, torch.float32, (q.shape[1], q.shape[0]))
+    given = _heads(op, "d_out", d_out, q, q.shape)
+    place = _heads(op, "out", out, q, q.shape)
+    (dq, dq_at), (dk, dk_at), (dv, dv_at) = _out(op, "dq", dq, q), _out(op, "dk", dk, k), _out(op, "dv", dv, v)
+    dtable = torch.empty_like(table) if table is not None else None
+    args, space = _with_space((*before, *place, *after, lse_at), q, 1)
+    _call(_lib.lib().ixh_attend_backward, q, args,
+          _GRADS.pack(*given, *dq_at, *dk_at, *dv_at, dtable.data_ptr() if dtable is not None else 0))
     return dq, dk, dv, dtable
 
 
@@ -172,28 +184,26 @@ def rel_buckets(buckets, max_distance, bidirectional=True):
 
 
 def _norm_rope_args(op, q, k, cos, sin, pos, q_gamma, k_gamma, norm, eps, pairs):
-    _rows(op, "q", q)
-    _rows(op, "k", k, q)
-    n, dim = q.shape[0], q.shape[2]
-    _need(k.shape[0] == n and k.shape[2] == dim, op, "q and k do not fit together")
+    """The values of ixh_norm_rope_args before and after q_out and k_out, up
+    to the workspace."""
+    qh, kh = _heads(op, "q", q), _heads(op, "k", k, q)
+    n, q_heads, dim = q.shape
+    n_k, k_heads, k_dim = k.shape
+    _need(n_k == n and k_dim == dim, op, "q and k do not fit together")
     _need(norm in _lib.HEAD_NORMS and pairs in _lib.PAIRS, op, f"norm {norm!r}, pairs {pairs!r}")
-    a = _lib.IxhNormRopeArgs()
-    a.type, a.n, a.q_heads, a.k_heads, a.dim = _TYPES[q.dtype], n, q.shape[1], k.shape[1], dim
-    a.q, a.k = _heads(q), _heads(k)
-    a.norm, a.eps, a.pairs = _lib.HEAD_NORMS[norm], eps, _lib.PAIRS[pairs]
     gamma = q_gamma if q_gamma is not None else k_gamma
     dtype = torch.float32 if gamma is None else gamma.dtype
     _need(dtype in _TYPES, op, f"gammas of type {dtype}")
-    a.gamma_type = _TYPES[dtype]
-    a.q_gamma = _plain(op, "q_gamma", q_gamma, q, dtype, (dim,))
-    a.k_gamma = _plain(op, "k_gamma", k_gamma, q, dtype, (dim,))
+    rows = rot = 0
     if cos is not None:
         _need(cos.dim() == 2 and sin is not None, op, "cos and sin are not [rows][columns / 2]")
-        a.rows, a.rot = cos.shape[0], 2 * cos.shape[1]
-        a.cos = _plain(op, "cos", cos, q, torch.float32, tuple(cos.shape))
-        a.sin = _plain(op, "sin", sin, q, torch.float32, tuple(cos.shape))
-    a.pos = _plain(op, "pos", pos, q, torch.int32, (n,))
-    return a
+        rows, rot = cos.shape[0], 2 * cos.shape[1]
+    return (_TYPES[q.dtype], n, q_heads, k_heads, dim, *qh, *kh), (
+        _lib.HEAD_NORMS[norm], eps, _TYPES[dtype],
+        _plain(op, "q_gamma", q_gamma, q, dtype, (dim,)), _plain(op, "k_gamma", k_gamma, q, dtype, (dim,)),
+        _plain(op, "cos", cos, q, torch.float32, (rows, rot // 2)),
+        _plain(op, "sin", sin, q, torch.float32, (rows, rot // 2)) if cos is not None else 0,
+        rows, rot, _lib.PAIRS[pairs], _plain(op, "pos", pos, q, torch.int32, (n,)))
 
 
 def qk_norm_rope(q, k, cos=None, sin=None, *, pos=None, q_gamma=None, k_gamma=None, norm="rms", eps=1e-6,
@@ -206,11 +216,9 @@ def qk_norm_rope(q, k, cos=None, sin=None, *, pos=None, q_gamma=None, k_gamma=No
     itself; a place past the tables gives NaN); pairs: "halves" (column i with
     i + columns / 2) or "neighbours" (2i with 2i + 1)."""
     op = "QKNormRope"
-    a = _norm_rope_args(op, q, k, cos, sin, pos, q_gamma, k_gamma, norm, eps, pairs)
-    q_out = _out(op, "q_out", q_out, q, tuple(q.shape))
-    k_out = _out(op, "k_out", k_out, q, tuple(k.shape))
-    a.q_out, a.k_out = _heads(q_out), _heads(k_out)
-    _lib.check(_lib.lib().ixh_qk_norm_rope(q.device.index, C.byref(a), _stream(q)))
+    before, after = _norm_rope_args(op, q, k, cos, sin, pos, q_gamma, k_gamma, norm, eps, pairs)
+    (q_out, q_at), (k_out, k_at) = _out(op, "q_out", q_out, q), _out(op, "k_out", k_out, k)
+    _call(_lib.lib().ixh_qk_norm_rope, q, _NORM_ROPE.pack(*before, *q_at, *k_at, *after, 0, 0))
     return q_out, k_out
 
 
@@ -220,22 +228,19 @@ def qk_norm_rope_backward(dq_out, dk_out, q, k, cos=None, sin=None, *, pos=None,
     arguments (q and k as they went in); a gamma's is None without it. dq and
     dk may be dq_out and dk_out themselves."""
     op = "QKNormRopeBackward"
-    a = _norm_rope_args(op, q, k, cos, sin, pos, q_gamma, k_gamma, norm, eps, pairs)
-    for name, t, like in (("dq_out", dq_out, q), ("dk_out", dk_out, k)):
-        _rows(op, name, t, q)
-        _need(t.shape == like.shape, op, f"{name} has another shape than its rows")
-    dq = _out(op, "dq", dq, q, tuple(q.shape))
-    dk = _out(op, "dk", dk, q, tuple(k.shape))
+    before, after = _norm_rope_args(op, q, k, cos, sin, pos, q_gamma, k_gamma, norm, eps, pairs)
+    given = (*_heads(op, "dq_out", dq_out, q, q.shape), *_heads(op, "dk_out", dk_out, q, k.shape))
+    (dq, dq_at), (dk, dk_at) = _out(op, "dq", dq, q), _out(op, "dk", dk, k)
     dq_gamma = None if q_gamma is None else torch.empty_like(q_gamma)
     dk_gamma = None if k_gamma is None else torch.empty_like(k_gamma)
-    g = _lib.IxhNormRopeGrads(_heads(dq_out), _heads(dk_out), _heads(dq), _heads(dk),
-                              None if dq_gamma is None else dq_gamma.data_ptr(),
-                              None if dk_gamma is None else dk_gamma.data_ptr())
-    space = None
+    none = (0, 0, 0)
+    args, space = (*before, *none, *none, *after), None
     if dq_gamma is not None or dk_gamma is not None:
         n = C.c_int64()
-        _lib.check(_lib.lib().ixh_qk_norm_rope_workspace(C.byref(a), C.byref(n)))
-        space = _space(q, n.value)
-        a.workspace, a.workspace_bytes = space.data_ptr(), n.value
-    _lib.check(_lib.lib().ixh_qk_norm_rope_backward(q.device.index, C.byref(a), C.byref(g), _stream(q)))
+        _lib.check(_lib.lib().ixh_qk_norm_rope_workspace(_NORM_ROPE.pack(*args, 0, 0), C.byref(n)))
+        space = _space(q, n.value)  # held until the call has queued its work
+    _call(_lib.lib().ixh_qk_norm_rope_backward, q,
+          _NORM_ROPE.pack(*args, space.data_ptr() if space is not None else 0, n.value if space is not None else 0),
+          _NORM_ROPE_GRADS.pack(*given, *dq_at, *dk_at, dq_gamma.data_ptr() if dq_gamma is not None else 0,
+                                dk_gamma.data_ptr() if dk_gamma is not None else 0))
     return dq, dk, dq_gamma, dk_gamma

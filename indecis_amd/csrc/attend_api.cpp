@@ -41,7 +41,8 @@ struct OnDevice {
   hipError_t err;
   explicit OnDevice(int dev) {
     if (hipGetDevice(&prev) != hipSuccess) prev = -1;
-    err = hipSetDevice(dev);
+    err = prev == dev ? hipSuccess : hipSetDevice(dev);
+    if (prev == dev) prev = -1;
   }
   ~OnDevice() {
     if (prev >= 0) (void)hipSetDevice(prev);

@@ -17,12 +17,12 @@ namespace {
 
 // z (base 2) of 16 scores, and under a cap its derivative by the score.
 template <class T, int FEAT>
-__device__ __forceinline__ void shape_scores(v16f &z, float *slope_of, const Score &sc, const Bias &by, const v16f &bias) {
+__device__ __forceinline__ void shape_scores(v16f &z, float *slope_of, const Score &sc, const v16f &bias) {
 #pragma unroll
   for (int r = 0; r < 16; r++) {
     if constexpr (FEAT & kCap) {
-      float u;
-      z[r] = capped<T>(sc, z[r], &u);
+      const float u = capped<T>(sc, z[r]);
+      z[r] = __builtin_fmaf(u, cap_gain(sc), sc.c2);
       slope_of[r] = 4.0f * u * (1.0f - u);
       if constexpr (FEAT & kBias) z[r] += bias[r];
     } else {
@@ -38,7 +38,7 @@ struct DqShape {
   static constexpr int WAVES = 4, THREADS = 256, ROWS = 128;
   static constexpr int BK = 32;
   typedef Tile<T, DT, BK, THREADS> KV;
-  static constexpr int DOCS = 4 * KV::BYTES, LIVE = DOCS + 2 * 4 * BK, BIAS = LIVE + 16 * kDocWords;
+  static constexpr int DOCS = 4 * KV::BYTES, LIVE = DOCS + 2 * 4 * BK, BIAS = LIVE + 8 * kDocWords;
 };
 
 template <class T, int DT, int FEAT>
@@ -52,7 +52,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : 2) void attend_dq_kernel(
   const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   int *const kdocs = (int *)(smem + Sh::DOCS);
-  uint64_t *const live = (uint64_t *)(smem + Sh::LIVE), *const pure = live + kDocWords;
+  uint64_t *const live = (uint64_t *)(smem + Sh::LIVE);
   float *const bias = (float *)(smem + Sh::BIAS);
   // sums of dZ by distance, an array each wave, with the bias' ends
   const int span = 2 * a.reach + 1, len = attend_bias_len(a.reach);
@@ -90,11 +90,12 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : 2) void attend_dq_kernel(
     t_end = u >= l ? u / BK + 1 : t_begin;
   }
   const int64_t row = s.q0 + tok;
-  const int doc = a.q_docs ? max(a.q_docs[row], -1) : 0;
+  const ColumnDocs docs(a.q_docs ? a.q_docs[row] : 0);
 
   // a row that sees nothing has lse -inf: its dO and o are not read
   const float lse = a.lse[(int64_t)head * a.nq + row];
   const bool alive = lse > -INFINITY;
+  const bool dead_rows = __ballot(!alive) != 0;
   const float lse2 = alive ? lse * kLog2e : 0.0f;
   Frag q[KS], dO[KS];
   float delta = 0.0f;
@@ -127,7 +128,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : 2) void attend_dq_kernel(
   }
   if (a.q_docs)
     doc_steps<BK, Sh::WAVES>(a.q_docs + s.q0, first, min(first + ROWS, s.nq) - 1, a.k_docs + s.k0, s.nk, t_begin, t_end,
-                             live, pure, wave, lane);
+                             live, wave, lane);
   if (a.q_docs || (FEAT & kBias)) __syncthreads();
   auto next = [&](int t) { return a.q_docs ? next_live(live, t, t_begin, t_end) : t; };
   float *const my_dist = dist + wave * len;
@@ -155,11 +156,10 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : 2) void attend_dq_kernel(
   if (t < t_end) fetch(t);
   for (int tn; t < t_end; t = tn, buf ^= 1) {
     char *const kl = smem + buf * 2 * KV::BYTES, *const vl = kl + KV::BYTES;
-    const bool docs = a.q_docs && !is_pure(pure, t - t_begin);
     {
-      const bool all = a.dim == DT && t * BK + BK <= s.nk && !docs;
-      auto keep = [&](int d) { return !docs || d >= 0; };
-      if (docs && tid < BK) kdocs[buf * BK + tid] = kdoc < 0 ? -2 : kdoc;
+      const bool all = a.dim == DT && t * BK + BK <= s.nk && !a.q_docs;
+      auto keep = [&](int d) { return !a.q_docs || d >= 0; };
+      if (a.q_docs && tid < BK) kdocs[buf * BK + tid] = kdoc < 0 ? -2 : kdoc;
       kt.put(kl, s.nk - t * BK, a.dim, tid, all, tags, keep);
       vt.put(vl, s.nk - t * BK, a.dim, tid, all, tags, keep);
     }
@@ -168,6 +168,12 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : 2) void attend_dq_kernel(
     if (tn < t_end) fetch(tn);
     const int j0 = t * BK;
     if (j0 > hi_max || j0 + BK <= lo_min) continue;
+    const bool masked = a.q_docs || j0 < lo_max || j0 + BK - 1 > hi_min || dead_rows;
+    unsigned bits = ~0u;
+    if (masked) {
+      bits = alive ? row_bits(j0, lo, hi, h) : 0;
+      if (a.q_docs && !docs.tile(kdocs + buf * BK, lane, &bits)) continue;
+    }
 
     const int d0 = j0 + 4 * h - p;
     const int near = j0 - p_hi, far = j0 + 31 - p_lo;
@@ -181,23 +187,13 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : 2) void attend_dq_kernel(
       dp = mfma16(KV::rows(vl, 0, i, lane), dO[i], dp);
     }
     float by_cap[16];
-    shape_scores<T, FEAT>(z, by_cap, sc, by, bz);
+    shape_scores<T, FEAT>(z, by_cap, sc, bz);
     float dz[16];
 #pragma unroll
     for (int r = 0; r < 16; r++) dz[r] = exp2_fast(z[r] - lse2) * (dp[r] - delta);
-    if (docs || j0 < lo_max || j0 + BK - 1 > hi_min || __ballot(!alive) != 0) {
-      const unsigned bits = alive ? row_bits(j0, lo, hi, h) : 0;
+    if (masked) {
 #pragma unroll
-      for (int r = 0; r < 16; r++) dz[r] = if_bit(bits, r, dz[r], 0);
-      if (docs) {
-#pragma unroll
-        for (int g = 0; g < 4; g++) {
-          const i4 d = *(const i4 *)(kdocs + buf * BK + 8 * g + 4 * h);
-#pragma unroll
-          for (int e = 0; e < 4; e++)
-            if (d[e] != doc) dz[4 * g + e] = 0.0f;
-        }
-      }
+      for (int r = 0; r < 16; r++) dz[r] = if_bit(bits, r, dz[r]);
     }
     if constexpr (FEAT & kBias) {
       if (grad_table) {
@@ -255,18 +251,10 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : 2) void attend_dq_kernel(
     }
   }
 
-  if (mine) {
-    T *o = (T *)x.g.dq.p + row * x.g.dq.row + head * x.g.dq.head;
-#pragma unroll
-    for (int d = 0; d < ND; d++)
-#pragma unroll
-      for (int g = 0; g < 4; g++) {
-        const int c = 32 * d + 8 * g + 4 * h;
-        if (c < a.dim)
-          store4(o + c, f4{acc[d][4 * g] * a.scale, acc[d][4 * g + 1] * a.scale, acc[d][4 * g + 2] * a.scale,
-                           acc[d][4 * g + 3] * a.scale});
-      }
-  }
+  store_rows<T, DT>(acc, a.scale, smem + wave * (32 * DT * (int)sizeof(T)), a.dim, lane, [&](int i) {
+    const int r = first + wave * 32 + i;
+    return r < s.nq ? (T *)x.g.dq.p + (int64_t)(s.q0 + r) * x.g.dq.row + head * x.g.dq.head : (T *)nullptr;
+  });
   if constexpr (FEAT & kBias) {
     if (grad_table) {
       // the ends: the lanes' sums in a fixed order, then the arrays past the
@@ -307,7 +295,7 @@ struct DkvShape {
   typedef Tile<T, DT, BQ, THREADS> QO;
   // Q and dO twice, then lse, delta and the documents of the rows twice
   static constexpr int STAT = 4 * QO::BYTES, DOCS = STAT + 4 * 4 * BQ, LIVE = DOCS + 2 * 4 * BQ,
-                       BIAS = LIVE + 16 * kDocWords;
+                       BIAS = LIVE + 8 * kDocWords;
 };
 
 template <class T, int DT, int FEAT>
@@ -322,7 +310,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 || DT == 128 ? 1 : 2) void atte
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   float *const stat = (float *)(smem + Sh::STAT);
   int *const qdocs = (int *)(smem + Sh::DOCS);
-  uint64_t *const live = (uint64_t *)(smem + Sh::LIVE), *const pure = live + kDocWords;
+  uint64_t *const live = (uint64_t *)(smem + Sh::LIVE);
   float *const bias = (float *)(smem + Sh::BIAS);
 
   const int kvh = blockIdx.x % a.kv_heads;
@@ -333,7 +321,6 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 || DT == 128 ? 1 : 2) void atte
   if (blk * KEYS >= s.nk) return;
   const int first = (int)(blk * KEYS);
   const int key = min(first + wave * 32 + (lane & 31), s.nk - 1);
-  const bool mine = first + wave * 32 + (lane & 31) < s.nk;
   int lo, hi;  // places of the queries that see the key
   query_bounds(a, s, key, &lo, &hi);
   const int k_lo = __builtin_amdgcn_readlane(key, 0), k_hi = __builtin_amdgcn_readlane(key, 31);
@@ -351,9 +338,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 || DT == 128 ? 1 : 2) void atte
     if (t_end < t_begin) t_end = t_begin;
   }
   const int64_t row = s.k0 + key;
-  const int kd = a.k_docs ? a.k_docs[row] : 0;
-  const int doc = kd < 0 ? -2 : kd;
-  const bool alive = !a.k_docs || kd >= 0;
+  const ColumnDocs docs(a.k_docs ? a.k_docs[row] : 0);
+  const bool alive = docs.doc >= 0;
 
   Frag k[KS], v[KS];
   {
@@ -368,7 +354,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 || DT == 128 ? 1 : 2) void atte
   }
   if (a.q_docs) {
     doc_steps<BQ, Sh::WAVES>(a.k_docs + s.k0, first, min(first + KEYS, s.nk) - 1, a.q_docs + s.q0, s.nq, t_begin, t_end,
-                             live, pure, wave, lane);
+                             live, wave, lane);
     __syncthreads();
   }
   auto next = [&](int t) { return a.q_docs ? next_live(live, t, t_begin, t_end) : t; };
@@ -415,14 +401,13 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 || DT == 128 ? 1 : 2) void atte
     for (int t = t_first, tn; t < t_end; t = tn, buf ^= 1) {
       char *const ql = smem + buf * 2 * QO::BYTES, *const gl = ql + QO::BYTES;
       float *const st = stat + buf * 2 * BQ;
-      const bool docs = a.q_docs && !is_pure(pure, t - t_begin);
       {
         // such rows, and those past the last, are cleared: P is 0 at +inf
         if (tid < BQ) {
           const bool there = lse > -INFINITY && t * BQ + tid < s.nq;
           st[tid] = there ? lse * kLog2e : INFINITY;
           st[BQ + tid] = there ? delta : 0.0f;
-          qdocs[buf * BQ + tid] = max(qdoc, -1);
+          qdocs[buf * BQ + tid] = qdoc < 0 ? -2 : qdoc;
         }
         auto keep = [&](int l) { return __builtin_bit_cast(float, l) > -INFINITY; };
         qt.put(ql, s.nq - t * BQ, a.dim, tid, false, tags, keep);
@@ -433,6 +418,12 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 || DT == 128 ? 1 : 2) void atte
       if (tn < t_end) fetch(tn);
       const int p0 = t * BQ + s.shift;  // place of the step's first query
       if (p0 > hi_max || p0 + BQ <= lo_min) continue;
+      const bool masked = a.q_docs || p0 < lo_max || p0 + BQ - 1 > hi_min;
+      unsigned bits = ~0u;
+      if (masked) {
+        bits = row_bits(p0, lo, hi, h);
+        if (a.q_docs && !docs.tile(qdocs + buf * BQ, lane, &bits)) continue;
+      }
 
       v16f z = v16f{}, dp = v16f{}, bz = v16f{};
       if constexpr (FEAT & kBias) bz = by.template at<-1>(key - p0 - 4 * h, k_lo - p0 - 31, k_hi - p0);
@@ -443,7 +434,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 || DT == 128 ? 1 : 2) void atte
         dp = mfma16(QO::rows(gl, 0, i, lane), v[i], dp);
       }
       float by_cap[16];
-      shape_scores<T, FEAT>(z, by_cap, sc, by, bz);
+      shape_scores<T, FEAT>(z, by_cap, sc, bz);
       float pr[16];
 #pragma unroll
       for (int g4 = 0; g4 < 4; g4++) {
@@ -451,19 +442,9 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 || DT == 128 ? 1 : 2) void atte
 #pragma unroll
         for (int e = 0; e < 4; e++) pr[4 * g4 + e] = exp2_fast(z[4 * g4 + e] - l[e]);
       }
-      if (docs || p0 < lo_max || p0 + BQ - 1 > hi_min) {
-        const unsigned bits = row_bits(p0, lo, hi, h);
+      if (masked) {
 #pragma unroll
-        for (int r = 0; r < 16; r++) pr[r] = if_bit(bits, r, pr[r], 0);
-        if (docs) {
-#pragma unroll
-          for (int g4 = 0; g4 < 4; g4++) {
-            const i4 d = *(const i4 *)(qdocs + buf * BQ + 8 * g4 + 4 * h);
-#pragma unroll
-            for (int e = 0; e < 4; e++)
-              if (d[e] != doc) pr[4 * g4 + e] = 0.0f;
-          }
-        }
+        for (int r = 0; r < 16; r++) pr[r] = if_bit(bits, r, pr[r]);
       }
       float ds[16];
 #pragma unroll
@@ -488,20 +469,15 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 || DT == 128 ? 1 : 2) void atte
       }
     }
   }
-  if (!mine) return;
-  T *ok = (T *)x.g.dk.p + row * x.g.dk.row + kvh * x.g.dk.head;
-  T *ov = (T *)x.g.dv.p + row * x.g.dv.row + kvh * x.g.dv.head;
-#pragma unroll
-  for (int d = 0; d < ND; d++)
-#pragma unroll
-    for (int g = 0; g < 4; g++) {
-      const int c = 32 * d + 8 * g + 4 * h;
-      if (c < a.dim) {
-        store4(ok + c, f4{dk[d][4 * g] * a.scale, dk[d][4 * g + 1] * a.scale, dk[d][4 * g + 2] * a.scale,
-                          dk[d][4 * g + 3] * a.scale});
-        store4(ov + c, f4{dv[d][4 * g], dv[d][4 * g + 1], dv[d][4 * g + 2], dv[d][4 * g + 3]});
-      }
-    }
+  auto to = [&](const ixh_heads &t) {
+    return [&, t](int i) {
+      const int r = first + wave * 32 + i;
+      return r < s.nk ? (T *)t.p + (int64_t)(s.k0 + r) * t.row + kvh * t.head : (T *)nullptr;
+    };
+  };
+  char *const mine_lds = smem + wave * (32 * DT * (int)sizeof(T));
+  store_rows<T, DT>(dk, a.scale, mine_lds, a.dim, lane, to(x.g.dk));
+  store_rows<T, DT>(dv, 1.0f, mine_lds, a.dim, lane, to(x.g.dv));
 }
 
 // ---- the table's gradient ----------------------------------------------------

@@ -149,9 +149,20 @@ __device__ __forceinline__ float lane_up(float v) {
 }
 
 // ---- tiles of rows in LDS ---------------------------------------------------
-// R rows of DT values, 16-byte pieces; piece c of row r stands at c ^ (r & 7),
-// so that the 16 rows a quarter-wave reads of one column of pieces, and the 8
-// rows a transposed read touches, lie in different banks.
+// R rows of DT values in 16-byte pieces; piece c of row r stands at
+// c ^ turn(r). A wave's read of rows takes 2 pieces of 32 rows, a transposed
+// one 4 pieces side by side of 8 rows. At 256 bytes a row the rows of one
+// transposed read are turned by whole groups of 4 pieces (every 16-byte slot
+// of the banks' 256 bytes is then asked equally often: a training step of 8
+// sequences of 2,048, 16/4 heads of 128, 898 -> 846 us against r & 7); at
+// 128 bytes two rows lie in one round of the banks and r & 7 is as good. A
+// turn is the same 8 rows on, so that the second half of a transposed read
+// is a constant offset.
+template <class T, int DT>
+__device__ __forceinline__ int turn(int r) {
+  if constexpr (sizeof(T) == 2 && DT == 128) return (r & 3) << 2 | (r >> 2 & 1);
+  return r & 7;
+}
 template <class T, int DT, int R, int THREADS>
 struct Tile {
   static constexpr int EPC = 16 / (int)sizeof(T);  // values a piece
@@ -201,7 +212,7 @@ struct Tile {
       const int r = tid / CH + i * STEP, c = tid % CH;
       i4 v = part[i];
       if (!all && !(c * EPC < dim && r < left && keep(tags.v[i]))) v = i4{0, 0, 0, 0};
-      *(i4 *)(lds + r * RB + ((c ^ (r & 7)) << 4)) = v;
+      *(i4 *)(lds + r * RB + ((c ^ turn<T, DT>(r)) << 4)) = v;
     }
   }
 
@@ -210,11 +221,11 @@ struct Tile {
     const int r = row0 + (lane & 31), h = lane >> 5;
     typename Kind<T>::frag f;
     if constexpr (sizeof(T) == 2) {
-      f = *(const typename Kind<T>::frag *)(lds + r * RB + (((2 * s + h) ^ (r & 7)) << 4));
+      f = *(const typename Kind<T>::frag *)(lds + r * RB + (((2 * s + h) ^ turn<T, DT>(r)) << 4));
     } else {
       const int c = 4 * s + 2 * h;
-      f.lo = *(const f4 *)(lds + r * RB + ((c ^ (r & 7)) << 4));
-      f.hi = *(const f4 *)(lds + r * RB + (((c + 1) ^ (r & 7)) << 4));
+      f.lo = *(const f4 *)(lds + r * RB + ((c ^ turn<T, DT>(r)) << 4));
+      f.hi = *(const f4 *)(lds + r * RB + (((c + 1) ^ turn<T, DT>(r)) << 4));
     }
     return f;
   }
@@ -226,7 +237,7 @@ struct Tile {
     if constexpr (sizeof(T) == 2) {
       const int a = lane & 15, g = (lane >> 4) & 1;
       const int r = row0 + 4 * h + (a >> 2), c = 4 * dt + 2 * g + ((a >> 1) & 1);
-      const char *p = lds + r * RB + ((c ^ (r & 7)) << 4) + ((a & 1) << 3);
+      const char *p = lds + r * RB + ((c ^ turn<T, DT>(r)) << 4) + ((a & 1) << 3);
       typedef __attribute__((address_space(3))) v4s lv4s;
       union {
         v4s q[2];
@@ -240,7 +251,7 @@ struct Tile {
 #pragma unroll
       for (int j = 0; j < 4; j++) {
         const int r = row0 + 4 * h + j;
-        const char *p = lds + r * RB + ((c ^ (r & 7)) << 4) + ((d & 3) << 2);
+        const char *p = lds + r * RB + ((c ^ turn<T, DT>(r)) << 4) + ((d & 3) << 2);
         f.lo[j] = *(const float *)p;
         f.hi[j] = *(const float *)(p + 8 * RB);
       }
@@ -248,6 +259,34 @@ struct Tile {
     return f;
   }
 };
+
+// A wave's 32 result rows (lane l has row l % 32, columns as the registers
+// hold them) times f, through 32 rows of its own in LDS to whole rows in
+// memory: eight bytes a lane of a row each would cost the address unit a
+// cycle a lane, 45 us of a launch of 9,864 blocks. row_at(i): the address of
+// row i, or nullptr. Every wave calls it, the block's tiles no longer needed.
+template <class T, int DT, class RowAt>
+__device__ __forceinline__ void store_rows(const v16f *acc, float f, char *lds, int dim, int lane, RowAt row_at) {
+  constexpr int EPC = 16 / (int)sizeof(T), CH = DT / EPC, RB = DT * (int)sizeof(T);
+  const int r = lane & 31, h = lane >> 5;
+  __syncthreads();
+#pragma unroll
+  for (int d = 0; d < DT / 32; d++)
+#pragma unroll
+    for (int g = 0; g < 4; g++) {
+      const int c = 32 * d + 8 * g + 4 * h;
+      store4((T *)(lds + r * RB + (((c / EPC) ^ turn<T, DT>(r)) << 4)) + c % EPC,
+             f4{acc[d][4 * g] * f, acc[d][4 * g + 1] * f, acc[d][4 * g + 2] * f, acc[d][4 * g + 3] * f});
+    }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 32 * CH / 64; i++) {
+    const int at = i * 64 + lane, row = at / CH, c = at % CH;
+    T *const to = row_at(row);
+    const i4 v = *(const i4 *)(lds + row * RB + ((c ^ turn<T, DT>(row)) << 4));
+    if (to && c * EPC < dim) *(i4 *)(to + c * EPC) = v;
+  }
+}
 
 // ---- sequences and masks ----------------------------------------------------
 
@@ -314,18 +353,15 @@ __device__ __forceinline__ void query_bounds(const ixh_attend_args &a, const Seq
 
 constexpr int kDocWords = 64;  // of 64 steps; later steps are taken as live
 
-// Which of the steps t0..t1 - 1 (`step` rows each, of the n in `theirs`) hold
-// a row of a document that a row first..last of `mine` has, and which hold
-// one document alone, that of all of mine (pure: no mask is needed). Every
-// wave calls it; a barrier before the words are read.
+// Which of the steps t0..t1 - 1 (STEP rows each, of the n in `theirs`) may
+// hold a row of a document that a row first..last of `mine` has. Every wave
+// calls it; a barrier before the words are read.
 template <int STEP, int WAVES>
 __device__ __forceinline__ void doc_steps(const int32_t *mine, int first, int last, const int32_t *theirs, int n, int t0,
-                                          int t1, uint64_t *live, uint64_t *pure, int wave, int lane) {
+                                          int t1, uint64_t *live, int wave, int lane) {
   int mn = INT32_MAX, mx = -1;
-  bool none = false;
   for (int i = first + lane; i <= last; i += 64) {
     const int d = mine[i];
-    none |= d < 0;
     mn = min(mn, d < 0 ? INT32_MAX : d);
     mx = max(mx, d);
   }
@@ -334,23 +370,19 @@ __device__ __forceinline__ void doc_steps(const int32_t *mine, int first, int la
     mn = min(mn, __shfl_xor(mn, o));
     mx = max(mx, __shfl_xor(mx, o));
   }
-  const bool one = mn == mx && !__ballot(none);
   for (int w = wave; w < kDocWords && t0 + 64 * w < t1; w += WAVES) {
     const int t = t0 + 64 * w + lane;
     int tmn = INT32_MAX, tmx = -1;
-    bool bad = t >= t1 || t * STEP + STEP > n;
     if (t < t1) {
 #pragma unroll
       for (int i = 0; i < STEP; i++) {
         const int d = theirs[min(t * STEP + i, n - 1)];
-        bad |= d < 0;
         tmn = min(tmn, d < 0 ? INT32_MAX : d);
         tmx = max(tmx, d);
       }
     }
-    const bool some = tmx >= 0 && mx >= 0 && tmn <= mx && tmx >= mn;
-    const uint64_t lv = __ballot(some), pr = __ballot(some && one && !bad && tmn == tmx && tmn == mn);
-    if (lane == 0) live[w] = lv, pure[w] = pr;
+    const uint64_t lv = __ballot(tmx >= 0 && mx >= 0 && tmn <= mx && tmx >= mn);
+    if (lane == 0) live[w] = lv;
   }
 }
 // The first live step from t on, t1 if none.
@@ -366,9 +398,44 @@ __device__ __forceinline__ int next_live(const uint64_t *live, int t, int t0, in
   }
   return t1;
 }
-__device__ __forceinline__ bool is_pure(const uint64_t *pure, int i) {
-  return i < 64 * kDocWords && __builtin_amdgcn_readfirstlane((int)(pure[i >> 6] >> (i & 63)) & 1);
-}
+
+// The documents of a wave's 32 columns.
+struct ColumnDocs {
+  int doc;   // the lane's: -1 for padding
+  int all;   // that of all of them,
+  bool one;  // if they have one
+  __device__ __forceinline__ explicit ColumnDocs(int d) {
+    doc = max(d, -1);
+    all = __builtin_amdgcn_readfirstlane(doc);
+    one = __ballot(doc == all) == ~0ull;
+  }
+  // Takes the lane's bits of the 32 rows whose documents stand at `rows` in
+  // LDS (padding: -2) that are of other documents out of `bits` (row_bits'
+  // order); whether any row is left to any lane. Where the columns or the
+  // rows have one document alone, that takes no comparison a score.
+  __device__ __forceinline__ bool tile(const int *rows, int lane, unsigned *bits) const {
+    const int h = lane >> 5, theirs = rows[lane & 31];
+    if (one) {
+      const unsigned hit = (unsigned)__ballot(theirs == all);
+      *bits &= hit >> (4 * h);
+      return hit != 0;
+    }
+    const int first = __builtin_amdgcn_readfirstlane(theirs);
+    if (__ballot(theirs == first) == ~0ull) {
+      if (doc != first) *bits = 0;
+      return __ballot(doc == first) != 0;
+    }
+    unsigned hit = 0;
+#pragma unroll
+    for (int g = 0; g < 4; g++) {
+      const i4 d = *(const i4 *)(rows + 8 * g + 4 * h);
+#pragma unroll
+      for (int e = 0; e < 4; e++) hit |= d[e] == doc ? 1u << (8 * g + e) : 0u;
+    }
+    *bits &= hit;
+    return true;
+  }
+};
 
 // ---- scores -----------------------------------------------------------------
 // FEAT: 1 a tanh cap, 2 a bias by distance.
@@ -389,22 +456,17 @@ struct Score {
   }
 };
 
-// c2 tanh(s c1): tanh(x) = 1 - 2u, u = 1 / (1 + e^2x), with the hardware's
-// exponential and reciprocal: off by about 1e-7 of 1, which next to a 16-bit
-// result is nothing; float32 takes the library's tanh. *u serves the
-// derivative, 1 - tanh^2 = 4 u (1 - u).
+// A capped score, c2 tanh(s c1), as c2 + cap_gain() * capped(): with
+// tanh(x) = 1 - 2u, u = 1 / (1 + e^2x), by the hardware's exponential and
+// reciprocal, off by about 1e-7 of 1, which next to a 16-bit result is
+// nothing. float32 takes the library's tanh, u = (1 - tanh) / 2. The
+// derivative is 1 - tanh^2 = 4 u (1 - u).
 template <class T>
-__device__ __forceinline__ float capped(const Score &sc, float s, float *u) {
-  if constexpr (sizeof(T) == 4) {
-    const float t = tanhf(s * sc.c1);
-    *u = 0.5f - 0.5f * t;
-    return sc.c2 * t;
-  } else {
-    const float e = exp2_fast(s * (sc.c1 * (2 * kLog2e)));
-    *u = __builtin_amdgcn_rcpf(1.0f + e);
-    return __builtin_fmaf(*u, -2.0f * sc.c2, sc.c2);
-  }
+__device__ __forceinline__ float capped(const Score &sc, float s) {
+  if constexpr (sizeof(T) == 4) return 0.5f - 0.5f * tanhf(s * sc.c1);
+  return __builtin_amdgcn_rcpf(1.0f + exp2_fast(s * (sc.c1 * (2 * kLog2e))));
 }
+__device__ __forceinline__ float cap_gain(const Score &sc) { return -2.0f * sc.c2; }
 
 // The bias starts the first product's sum, in units of q.k (bias / scale), so
 // that it costs no operation of its own; under a cap it is added to z, in
@@ -462,12 +524,16 @@ __device__ __forceinline__ unsigned row_bits(int j0, int lo, int hi, int h) {
   const unsigned below = (unsigned)((1ull << l) - 1), upto = (unsigned)((1ull << u) - 1);
   return (upto & ~below) >> (4 * h);
 }
-// v where the bit of register r is set, else `other`.
-__device__ __forceinline__ float if_bit(unsigned bits, int r, float v, unsigned other) {
+// v where the bit of register r is set, else -inf.
+__device__ __forceinline__ float or_minus_inf(unsigned bits, int r, float v) {
   const unsigned m = (unsigned)__builtin_amdgcn_sbfe((int)bits, 8 * (r >> 2) + (r & 3), 1);
-  return __builtin_bit_cast(float, (__builtin_bit_cast(unsigned, v) & m) | (other & ~m));
+  return __builtin_bit_cast(float, (__builtin_bit_cast(unsigned, v) & m) | (0xff800000u & ~m));
 }
-constexpr unsigned kMinusInf = 0xff800000u;
+// v where the bit of register r is set, else 0.
+__device__ __forceinline__ float if_bit(unsigned bits, int r, float v) {
+  const unsigned m = (unsigned)__builtin_amdgcn_sbfe((int)bits, 8 * (r >> 2) + (r & 3), 1);
+  return __builtin_bit_cast(float, __builtin_bit_cast(unsigned, v) & m);
+}
 
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float d;

@@ -16,11 +16,12 @@ namespace {
 template <class T, int DT, int WAVES>
 struct FwdShape {
   static constexpr int THREADS = 64 * WAVES, ROWS = 32 * WAVES;
-  static constexpr int BK = attend_keys(sizeof(T), WAVES == 1), NS = BK / 32;
+  static constexpr int BK = attend_keys(sizeof(T), WAVES == 1);
   typedef Tile<T, DT, BK, THREADS> KV;
-  // LDS: K and V twice, the key documents twice, the live and the pure steps
-  // of documents, then the bias
-  static constexpr int DOCS = 4 * KV::BYTES, LIVE = DOCS + 2 * 4 * BK, BIAS = LIVE + 16 * kDocWords;
+  static_assert(4 * KV::BYTES >= WAVES * 32 * DT * (int)sizeof(T), "the result's rows");
+  // LDS: K and V twice, the key documents twice, the live steps of documents,
+  // then the bias
+  static constexpr int DOCS = 4 * KV::BYTES, LIVE = DOCS + 2 * 4 * BK, BIAS = LIVE + 8 * kDocWords;
 };
 
 template <class T, int DT, int WAVES, int FEAT>
@@ -29,13 +30,13 @@ void attend_fwd_kernel(AttendArgs x) {
   typedef FwdShape<T, DT, WAVES> Sh;
   typedef typename Sh::KV KV;
   typedef typename Kind<T>::frag Frag;
-  constexpr int THREADS = Sh::THREADS, ROWS = Sh::ROWS, BK = Sh::BK, NS = Sh::NS, KS = DT / 16, ND = DT / 32;
+  constexpr int THREADS = Sh::THREADS, ROWS = Sh::ROWS, BK = Sh::BK, KS = DT / 16, ND = DT / 32;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const ixh_attend_args &a = x.a;
   const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   int *const kdocs = (int *)(smem + Sh::DOCS);
-  uint64_t *const live = (uint64_t *)(smem + Sh::LIVE), *const pure = live + kDocWords;
+  uint64_t *const live = (uint64_t *)(smem + Sh::LIVE);
   float *const bias = (float *)(smem + Sh::BIAS);
 
   // last blocks first: under a causal mask they have the most keys
@@ -79,14 +80,10 @@ void attend_fwd_kernel(AttendArgs x) {
     }
   }
 
-  // documents: which steps hold a key of one of this block's, and which hold
-  // one document only, this block's
-  int doc = 0;
-  if (a.q_docs) {
-    doc = max(a.q_docs[s.q0 + tok], -1);
+  const ColumnDocs docs(a.q_docs ? a.q_docs[s.q0 + tok] : 0);
+  if (a.q_docs)
     doc_steps<BK, WAVES>(a.q_docs + s.q0, (int)(blk * ROWS / pack), (int)((min(blk * ROWS + ROWS, rows) - 1) / pack),
-                         a.k_docs + s.k0, s.nk, t_begin, t_end, live, pure, wave, lane);
-  }
+                         a.k_docs + s.k0, s.nk, t_begin, t_end, live, wave, lane);
   if constexpr (FEAT & kBias) {
     if (a.table)
       for (int i = 0; i < pack; i++)
@@ -112,7 +109,8 @@ void attend_fwd_kernel(AttendArgs x) {
   v16f acc[ND];
 #pragma unroll
   for (int d = 0; d < ND; d++) acc[d] = v16f{};
-  float m = -INFINITY, ref = 0.0f, sum = 0.0f;  // maximum so far; what scores are taken against
+  // the maximum so far; what scores are taken against
+  float m = -INFINITY, ref = 0.0f, sum = 0.0f;
 
   KV kt, vt;
   typename KV::Tags tags;
@@ -129,58 +127,63 @@ void attend_fwd_kernel(AttendArgs x) {
     }
   };
 
-  // N 32-key tiles from key j0 of the sequence, rows r0 of the step in LDS:
+  // The 32 keys from key j0 of the sequence, row r0 of the step in LDS:
   // scores, running maximum and sum, and their part of the output.
-  auto tiles = [&](auto count, int j0, int r0, const char *kl, const char *vl, const int *kd) {
-    constexpr int N = count.value;
-    v16f z[N];
-#pragma unroll
-    for (int u = 0; u < N; u++) {
-      z[u] = v16f{};
-      if constexpr (FEAT == kBias) z[u] = by.template at<1>(j0 + 32 * u + 4 * h - p, j0 + 32 * u - p_hi, j0 + 32 * u + 31 - p_lo);
-#pragma unroll
-      for (int i = 0; i < KS; i++) z[u] = mfma16(KV::rows(kl, r0 + 32 * u, i, lane), q[i], z[u]);
+  auto tile = [&](int j0, int r0, const char *kl, const char *vl, const int *kd) {
+    const bool masked = kd || j0 < lo_max || j0 + 31 > hi_min;
+    unsigned bits = ~0u;
+    if (masked) {
+      bits = row_bits(j0, lo, hi, h);
+      if (kd && !docs.tile(kd + r0, lane, &bits)) return;
     }
-    const bool masked = kd || j0 < lo_max || j0 + 32 * N - 1 > hi_min;
+    const int d0 = j0 + 4 * h - p, near = j0 - p_hi, far = j0 + 31 - p_lo;
+    // a score is z * gain + c2 in base 2
+    v16f z{};
+    float gain = sc.c1;
+    if constexpr (FEAT == kBias) z = by.template at<1>(d0, near, far);
+#pragma unroll
+    for (int i = 0; i < KS; i++) z = mfma16(KV::rows(kl, r0, i, lane), q[i], z);
     if constexpr (FEAT & kCap) {
 #pragma unroll
-      for (int u = 0; u < N; u++) {
+      for (int r = 0; r < 16; r++) z[r] = capped<T>(sc, z[r]);
+      gain = cap_gain(sc);
+      if constexpr (FEAT & kBias) {
+        const v16f b = by.template at<1>(d0, near, far);
 #pragma unroll
-        for (int r = 0; r < 16; r++) {
-          float unused;
-          z[u][r] = capped<T>(sc, z[u][r], &unused);
-        }
-        if constexpr (FEAT & kBias)
-          z[u] += by.template at<1>(j0 + 32 * u + 4 * h - p, j0 + 32 * u - p_hi, j0 + 32 * u + 31 - p_lo);
+        for (int r = 0; r < 16; r++) z[r] = __builtin_fmaf(z[r], gain, b[r]);
+        gain = 1.0f;
       }
     }
-    if (masked) {
+    // The probabilities are taken against an old maximum until they add up
+    // to over 2^8: far inside every type's range, so few tiles after a
+    // query's first need their own maximum or rescale the sums.
+    float part, pr[16];
+    auto probabilities = [&] {
+      const float less = sc.c2 - ref;
+      part = 0.0f;
 #pragma unroll
-      for (int u = 0; u < N; u++) {
-        const unsigned bits = row_bits(j0 + 32 * u, lo, hi, h);
+      for (int r = 0; r < 16; r++) pr[r] = exp2_fast(__builtin_fmaf(z[r], gain, less));
+      if (masked) {
 #pragma unroll
-        for (int r = 0; r < 16; r++) z[u][r] = if_bit(bits, r, z[u][r], kMinusInf);
-        if (kd) {
-#pragma unroll
-          for (int g = 0; g < 4; g++) {
-            const i4 d = *(const i4 *)(kd + r0 + 32 * u + 8 * g + 4 * h);
-#pragma unroll
-            for (int e = 0; e < 4; e++)
-              if (d[e] != doc) z[u][4 * g + e] = -INFINITY;
-          }
-        }
+        for (int r = 0; r < 16; r++) pr[r] = if_bit(bits, r, pr[r]);
       }
-    }
-    float top = z[0][0];
 #pragma unroll
-    for (int u = 0; u < N; u++)
+      for (int r = 0; r < 16; r++) part += pr[r];
+      return __ballot(!(part <= 256.0f)) != 0;
+    };
+    bool again = __ballot(bits != 0 && m == -INFINITY) != 0;
+    if (!again) again = probabilities();
+    if (again) {
+      float top = -INFINITY, y[16];
 #pragma unroll
-      for (int r = 0; r < 16; r += 2) top = max3(z[u][r], z[u][r + 1], top);
-    top = half_max(top);
-    if constexpr (!(FEAT & kCap)) top *= sc.c1;
-    // the sums keep an old maximum until it is 2^8 short: they stay far
-    // inside every type's range, and few steps rescale
-    if (__ballot(top > m + 8.0f)) {
+      for (int r = 0; r < 16; r++) y[r] = __builtin_fmaf(z[r], gain, sc.c2);
+      if (masked) {
+#pragma unroll
+        for (int r = 0; r < 16; r++) y[r] = or_minus_inf(bits, r, y[r]);
+      }
+#pragma unroll
+      for (int r = 0; r < 16; r += 2) top = max3(y[r], y[r + 1], top);
+      top = half_max(top);
       const float next_m = __builtin_fmaxf(m, top);
       const float f = m == -INFINITY ? 0.0f : exp2_fast(m - next_m);
       m = next_m;
@@ -190,24 +193,16 @@ void attend_fwd_kernel(AttendArgs x) {
       for (int d = 0; d < ND; d++)
 #pragma unroll
         for (int r = 0; r < 16; r++) acc[d][r] *= f;
+      probabilities();
     }
+    sum += part;
+    // the probabilities are rounded to the rows' type here, as V is: the
+    // product's sum stays in 32 bits
 #pragma unroll
-    for (int u = 0; u < N; u++) {
-      float part = 0.0f, pr[16];
+    for (int v = 0; v < 2; v++) {
+      const Frag pf = pack8<Frag>(pr + 8 * v);
 #pragma unroll
-      for (int r = 0; r < 16; r++) {
-        pr[r] = exp2_fast((FEAT & kCap) ? z[u][r] - ref : __builtin_fmaf(z[u][r], sc.c1, -ref));
-        part += pr[r];
-      }
-      sum += part;
-      // the probabilities are rounded to the rows' type here, as V is: the
-      // product's sum stays in 32 bits
-#pragma unroll
-      for (int v = 0; v < 2; v++) {
-        const Frag pf = pack8<Frag>(pr + 8 * v);
-#pragma unroll
-        for (int d = 0; d < ND; d++) acc[d] = mfma16(KV::cols(vl, r0 + 32 * u + 16 * v, d, lane), pf, acc[d]);
-      }
+      for (int d = 0; d < ND; d++) acc[d] = mfma16(KV::cols(vl, r0 + 16 * v, d, lane), pf, acc[d]);
     }
   };
 
@@ -216,12 +211,11 @@ void attend_fwd_kernel(AttendArgs x) {
   if (t < t_end) fetch(t);
   while (t < t_end) {
     char *const kl = smem + buf * 2 * KV::BYTES, *const vl = kl + KV::BYTES;
-    const bool docs = a.q_docs && !is_pure(pure, t - t_begin);
     {
       // padding that no query sees may hold anything: its rows are cleared
-      const bool all = a.dim == DT && t * BK + BK <= s.nk && !docs;
-      auto keep = [&](int d) { return !docs || d >= 0; };
-      if (docs && tid < BK) kdocs[buf * BK + tid] = kdoc < 0 ? -2 : kdoc;
+      const bool all = a.dim == DT && t * BK + BK <= s.nk && !a.q_docs;
+      auto keep = [&](int d) { return !a.q_docs || d >= 0; };
+      if (a.q_docs && tid < BK) kdocs[buf * BK + tid] = kdoc < 0 ? -2 : kdoc;
       kt.put(kl, s.nk - t * BK, a.dim, tid, all, tags, keep);
       vt.put(vl, s.nk - t * BK, a.dim, tid, all, tags, keep);
     }
@@ -230,30 +224,19 @@ void attend_fwd_kernel(AttendArgs x) {
     if (tn < t_end) fetch(tn);
 
     const int j0 = t * BK;
-    const int *const kd = docs ? kdocs + buf * BK : nullptr;
-    auto live_at = [&](int j) { return j <= hi_max && j + 31 >= lo_min; };
-    if constexpr (NS == 1) {
-      if (live_at(j0)) tiles(std::integral_constant<int, 1>(), j0, 0, kl, vl, kd);
-    } else if constexpr (DT > 64) {
-      // one at a time: two tiles' scores beside 64 sums spill
+    const int *const kd = a.q_docs ? kdocs + buf * BK : nullptr;
+    // a tile at a time: two tiles' scores cost a wave of every SIMD
 #pragma unroll 1
-      for (int u = 0; u < 2; u++)
-        if (live_at(j0 + 32 * u)) tiles(std::integral_constant<int, 1>(), j0 + 32 * u, 32 * u, kl, vl, kd);
-    } else {
-      const bool first = live_at(j0), last = live_at(j0 + 32);
-      if (first && last)
-        tiles(std::integral_constant<int, 2>(), j0, 0, kl, vl, kd);
-      else if (first || last)
-        tiles(std::integral_constant<int, 1>(), last ? j0 + 32 : j0, last ? 32 : 0, kl, vl, kd);
-    }
+    for (int u = 0; u < BK; u += 32)
+      if (j0 + u <= hi_max && j0 + u + 31 >= lo_min) tile(j0 + u, u, kl, vl, kd);
     buf ^= 1;
     t = tn;
   }
 
   sum = half_sum(sum);
-  if (!mine) return;
   const int64_t row = s.q0 + tok;
   if (x.splits > 1) {
+    if (!mine) return;
     const int64_t at = ((int64_t)blockIdx.y * a.nq + row) * a.heads + head;
     float *o = x.part_o + at * a.dim;
 #pragma unroll
@@ -266,17 +249,13 @@ void attend_fwd_kernel(AttendArgs x) {
     if (h == 0) x.part_ml[2 * at] = m, x.part_ml[2 * at + 1] = sum;
     return;
   }
-  const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
-  T *o = (T *)a.o.p + row * a.o.row + head * a.o.head;
-#pragma unroll
-  for (int d = 0; d < ND; d++)
-#pragma unroll
-    for (int g = 0; g < 4; g++) {
-      const int c = 32 * d + 8 * g + 4 * h;
-      if (c < a.dim)
-        store4(o + c, f4{acc[d][4 * g] * inv, acc[d][4 * g + 1] * inv, acc[d][4 * g + 2] * inv, acc[d][4 * g + 3] * inv});
-    }
-  if (a.lse && h == 0) a.lse[(int64_t)head * a.nq + row] = (ref + __builtin_amdgcn_logf(sum)) * kLn2;
+  if (a.lse && mine && h == 0) a.lse[(int64_t)head * a.nq + row] = (ref + __builtin_amdgcn_logf(sum)) * kLn2;
+  store_rows<T, DT>(acc, sum > 0.0f ? 1.0f / sum : 0.0f, smem + wave * (32 * DT * (int)sizeof(T)), a.dim, lane, [&](int i) {
+    const int64_t r = blk * ROWS + wave * 32 + i;
+    if (r >= rows) return (T *)nullptr;
+    const int tok = pack > 1 ? (int)((unsigned)r / (unsigned)pack) : (int)r;
+    return (T *)a.o.p + (s.q0 + tok) * a.o.row + (pack > 1 ? hb * pack + (int)(r - (int64_t)tok * pack) : hb) * a.o.head;
+  });
 }
 
 // The parts of the keys joined: a thread has four columns of a query's head.
