@@ -71,7 +71,8 @@ def _plain(op, name, t, like, dtype, shape):
 def _out(op, name, t, like):
     """An output of like's shape, and its place."""
     if t is None:
-        t = torch.empty(like.shape, dtype=like.dtype, device=like.device)
+        t = like.new_empty(like.shape)
+        return t, (t.data_ptr(), t.stride(0), t.stride(1))
     return t, _heads(op, name, t, like, like.shape)
 
 
@@ -90,8 +91,8 @@ def _attend_args(op, q, k, v, offs, k_offs, scale, cap, slopes, table, buckets, 
     nq, heads, dim = q.shape
     nk, kv_heads, k_dim = k.shape
     _need(k.shape == v.shape and k_dim == dim, op, "q, k and v do not fit together")
-    _need(offs.dim() == 1 and len(offs) >= 1, op, "offs is not [sequences + 1]")
-    B = len(offs) - 1
+    B = offs.numel() - 1
+    _need(B >= 0, op, "offs is not [sequences + 1]")
     n_buckets = reach = 0
     if table is not None:
         _need(table.dim() == 2 and buckets is not None and buckets.dim() == 1 and len(buckets) % 2 == 1, op,
@@ -190,20 +191,21 @@ def _norm_rope_args(op, q, k, cos, sin, pos, q_gamma, k_gamma, norm, eps, pairs)
     n, q_heads, dim = q.shape
     n_k, k_heads, k_dim = k.shape
     _need(n_k == n and k_dim == dim, op, "q and k do not fit together")
-    _need(norm in _lib.HEAD_NORMS and pairs in _lib.PAIRS, op, f"norm {norm!r}, pairs {pairs!r}")
+    if norm not in _lib.HEAD_NORMS or pairs not in _lib.PAIRS:
+        _need(False, op, f"norm {norm!r}, pairs {pairs!r}")
     gamma = q_gamma if q_gamma is not None else k_gamma
     dtype = torch.float32 if gamma is None else gamma.dtype
-    _need(dtype in _TYPES, op, f"gammas of type {dtype}")
-    rows = rot = 0
+    _need(dtype in _TYPES, op, "gammas of another type than float32 and the rows'")
+    rows = half = 0
     if cos is not None:
         _need(cos.dim() == 2 and sin is not None, op, "cos and sin are not [rows][columns / 2]")
-        rows, rot = cos.shape[0], 2 * cos.shape[1]
+        rows, half = cos.shape
     return (_TYPES[q.dtype], n, q_heads, k_heads, dim, *qh, *kh), (
         _lib.HEAD_NORMS[norm], eps, _TYPES[dtype],
         _plain(op, "q_gamma", q_gamma, q, dtype, (dim,)), _plain(op, "k_gamma", k_gamma, q, dtype, (dim,)),
-        _plain(op, "cos", cos, q, torch.float32, (rows, rot // 2)),
-        _plain(op, "sin", sin, q, torch.float32, (rows, rot // 2)) if cos is not None else 0,
-        rows, rot, _lib.PAIRS[pairs], _plain(op, "pos", pos, q, torch.int32, (n,)))
+        _plain(op, "cos", cos, q, torch.float32, (rows, half)),
+        _plain(op, "sin", sin, q, torch.float32, (rows, half)) if cos is not None else 0,
+        rows, 2 * half, _lib.PAIRS[pairs], _plain(op, "pos", pos, q, torch.int32, (n,)))
 
 
 def qk_norm_rope(q, k, cos=None, sin=None, *, pos=None, q_gamma=None, k_gamma=None, norm="rms", eps=1e-6,

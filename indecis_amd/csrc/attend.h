@@ -39,6 +39,9 @@ constexpr int attend_keys(int size, bool few) { return size == 4 || few ? 32 : 6
 constexpr int kBiasPad = 96;
 constexpr int attend_bias_len(int reach) { return 2 * (reach + kBiasPad) + 1; }
 
+// Keys a workgroup of the dK, dV kernel.
+constexpr int attend_dkv_keys(int type_size, int dim) { return (type_size == 2) == (dim > 64) ? 64 : 128; }
+
 bool launch_attend_fwd(const AttendArgs &x, bool few, hipStream_t s);
 void launch_attend_join(const AttendArgs &x, hipStream_t s);
 bool launch_attend_dq(const AttendArgs &x, hipStream_t s);

@@ -233,7 +233,7 @@ int ixh_attend_backward(int device, const ixh_attend_args *a, const ixh_attend_g
       return rc;
   }
   const int64_t need = plan_backward(x);
-  const int64_t key_slots = attend_slots(a->nk, a->B, 128, 1);
+  const int64_t key_slots = attend_slots(a->nk, a->B, attend_dkv_keys(type_size(a->type), a->dim), 1);
   if (x.slots * a->heads > kMaxGrid || key_slots * a->kv_heads > kMaxGrid)
     return fail(IXH_EINVAL, "linalg: AttendBackward: too many rows and heads for one launch");
   if ((rc = check_workspace("AttendBackward", a->workspace, a->workspace_bytes, need))) return rc;

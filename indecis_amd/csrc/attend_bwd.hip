@@ -15,20 +15,19 @@
 namespace ixh {
 namespace {
 
-// z (base 2) of 16 scores, and under a cap its derivative by the score.
+// 16 products to scores: a score is then z * gain + c2 (Score's) in base 2.
+// Under a cap slope_of gets its derivative by the product, in units of scale.
 template <class T, int FEAT>
-__device__ __forceinline__ void shape_scores(v16f &z, float *slope_of, const Score &sc, const v16f &bias) {
+__device__ __forceinline__ float shape_scores(v16f &z, float *slope_of, const Score &sc, const v16f &bias) {
+  if constexpr (!(FEAT & kCap)) return sc.c1;
+  const float gain = cap_gain(sc);
 #pragma unroll
   for (int r = 0; r < 16; r++) {
-    if constexpr (FEAT & kCap) {
-      const float u = capped<T>(sc, z[r]);
-      z[r] = __builtin_fmaf(u, cap_gain(sc), sc.c2);
-      slope_of[r] = 4.0f * u * (1.0f - u);
-      if constexpr (FEAT & kBias) z[r] += bias[r];
-    } else {
-      z[r] *= sc.c1;
-    }
+    const float u = capped<T>(sc, z[r]);
+    z[r] = FEAT & kBias ? __builtin_fmaf(u, gain, bias[r]) : u;
+    slope_of[r] = 4.0f * u * (1.0f - u);
   }
+  return FEAT & kBias ? 1.0f : gain;
 }
 
 // ---- dQ ---------------------------------------------------------------------
@@ -42,7 +41,7 @@ struct DqShape {
 };
 
 template <class T, int DT, int FEAT>
-__global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : 2) void attend_dq_kernel(AttendArgs x) {
+__global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : DT == 64 ? 3 : 2) void attend_dq_kernel(AttendArgs x) {
   typedef DqShape<T, DT> Sh;
   typedef typename Sh::KV KV;
   typedef typename Kind<T>::frag Frag;
@@ -60,10 +59,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : 2) void attend_dq_kernel(
 
   const int head = blockIdx.x % a.heads, kvh = head / x.group;
   const int64_t slot = x.slots - 1 - blockIdx.x / a.heads;
-  int b;
   int64_t blk;
-  find_block(a.q_offs, a.B, a.nq, ROWS, 1, slot, &b, &blk);
-  const Seq s(a, b);
+  const Seq s = find_block(a, false, ROWS, 1, slot, &blk);
   const bool grad_table = (FEAT & kBias) && x.dist;
   float *const dist_out = grad_table ? x.dist + (slot * a.heads + head) * span : nullptr;
   if (blk * ROWS >= s.nq) {
@@ -118,6 +115,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : 2) void attend_dq_kernel(
   const T *const kb = (const T *)a.k.p + s.k0 * a.k.row + kvh * a.k.head;
   const T *const vb = (const T *)a.v.p + s.k0 * a.v.row + kvh * a.v.head;
   const Score sc(a, FEAT & kCap);
+  const float less = sc.c2 - lse2;
   const float unit = bias_unit(a, FEAT & kCap);
   const Bias by{(FEAT & kBias) && a.table ? bias : nullptr,
                 (FEAT & kBias) && a.slopes ? -a.slopes[head] * unit : 0.0f, a.reach};
@@ -182,15 +180,16 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : 2) void attend_dq_kernel(
     if constexpr (FEAT & kBias) bz = by.template at<1>(d0, near, far);
     if constexpr (FEAT == kBias) z = bz;
 #pragma unroll
-    for (int i = 0; i < KS; i++) {
-      z = mfma16(KV::rows(kl, 0, i, lane), q[i], z);
-      dp = mfma16(KV::rows(vl, 0, i, lane), dO[i], dp);
-    }
+    for (int i = 0; i < KS; i++)
+      if (within<T>(16 * i, a.dim)) {
+        z = mfma16(KV::rows(kl, 0, i, lane), q[i], z);
+        dp = mfma16(KV::rows(vl, 0, i, lane), dO[i], dp);
+      }
     float by_cap[16];
-    shape_scores<T, FEAT>(z, by_cap, sc, bz);
+    const float gain = shape_scores<T, FEAT>(z, by_cap, sc, bz);
     float dz[16];
 #pragma unroll
-    for (int r = 0; r < 16; r++) dz[r] = exp2_fast(z[r] - lse2) * (dp[r] - delta);
+    for (int r = 0; r < 16; r++) dz[r] = exp2_fast(__builtin_fmaf(z[r], gain, less)) * (dp[r] - delta);
     if (masked) {
 #pragma unroll
       for (int r = 0; r < 16; r++) dz[r] = if_bit(bits, r, dz[r]);
@@ -247,7 +246,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : 2) void attend_dq_kernel(
     for (int v = 0; v < 2; v++) {
       const Frag f = pack8<Frag>(dz + 8 * v);
 #pragma unroll
-      for (int d = 0; d < ND; d++) acc[d] = mfma16(KV::cols(kl, 16 * v, d, lane), f, acc[d]);
+      for (int d = 0; d < ND; d++)
+        if (within<T>(32 * d, a.dim)) acc[d] = mfma16(KV::cols(kl, 16 * v, d, lane), f, acc[d]);
     }
   }
 
@@ -288,10 +288,18 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : 2) void attend_dq_kernel(
 
 // ---- dK, dV -----------------------------------------------------------------
 
+// Four waves have 128 keys, 32 each, and 32 queries a step. Where the sums of
+// a wave take the registers of a whole SIMD (head dimensions over 64, or
+// float32), few blocks run at once, and a block of keys that many queries see
+// holds up the launch: there two waves share 32 keys, each with every other
+// 32 queries of a step of 64, and add their sums up at the end (8 sequences
+// of 2,048, 16/4 heads of 128, documents of up to 1,500: 441 -> 260 us).
 template <class T, int DT>
 struct DkvShape {
-  static constexpr int WAVES = 4, THREADS = 256, KEYS = 128;
-  static constexpr int BQ = 32;
+  static constexpr int SHARE = (sizeof(T) == 2) == (DT == 128) ? 2 : 1;
+  static constexpr int WAVES = 4, THREADS = 256, KEYS = 128 / SHARE;
+  static constexpr int BQ = 32 * SHARE;
+  static_assert(KEYS == attend_dkv_keys(sizeof(T), DT), "");
   typedef Tile<T, DT, BQ, THREADS> QO;
   // Q and dO twice, then lse, delta and the documents of the rows twice
   static constexpr int STAT = 4 * QO::BYTES, DOCS = STAT + 4 * 4 * BQ, LIVE = DOCS + 2 * 4 * BQ,
@@ -308,25 +316,24 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 || DT == 128 ? 1 : 2) void atte
   const ixh_attend_args &a = x.a;
   const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int kw = wave / Sh::SHARE, qw = wave % Sh::SHARE;  // the wave's keys, its queries of a step
   float *const stat = (float *)(smem + Sh::STAT);
   int *const qdocs = (int *)(smem + Sh::DOCS);
   uint64_t *const live = (uint64_t *)(smem + Sh::LIVE);
   float *const bias = (float *)(smem + Sh::BIAS);
 
   const int kvh = blockIdx.x % a.kv_heads;
-  int b;
   int64_t blk;
-  find_block(a.k_offs, a.B, a.nk, KEYS, 1, blockIdx.x / a.kv_heads, &b, &blk);
-  const Seq s(a, b);
+  const Seq s = find_block(a, true, KEYS, 1, blockIdx.x / a.kv_heads, &blk);
   if (blk * KEYS >= s.nk) return;
   const int first = (int)(blk * KEYS);
-  const int key = min(first + wave * 32 + (lane & 31), s.nk - 1);
+  const int key = min(first + kw * 32 + (lane & 31), s.nk - 1);
   int lo, hi;  // places of the queries that see the key
   query_bounds(a, s, key, &lo, &hi);
   const int k_lo = __builtin_amdgcn_readlane(key, 0), k_hi = __builtin_amdgcn_readlane(key, 31);
   const int lo_min = __builtin_amdgcn_readlane(lo, 0), lo_max = __builtin_amdgcn_readlane(lo, 31);
   const int hi_min = __builtin_amdgcn_readlane(hi, 0);
-  const int hi_max = first + wave * 32 < s.nk ? __builtin_amdgcn_readlane(hi, 31) : INT32_MIN;
+  const int hi_max = first + kw * 32 < s.nk ? __builtin_amdgcn_readlane(hi, 31) : INT32_MIN;
   int t_begin, t_end;  // steps of BQ queries
   {
     int l, u, unused;
@@ -364,115 +371,160 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 || DT == 128 ? 1 : 2) void atte
 #pragma unroll
   for (int d = 0; d < ND; d++) dk[d] = v16f{}, dv[d] = v16f{};
 
-  QO qt, gt;
-  typename QO::Tags tags;
-  qt.init(a.q.row, a.dim, tid);
-  gt.init(x.g.d_out.row, a.dim, tid);
-  float lse = 0.0f, delta = 0.0f;
-  int qdoc = 0, buf = 0;
-  for (int g = 0; g < x.group; g++) {
-    const int head = kvh * x.group + g;
-    const T *const qb = (const T *)a.q.p + s.q0 * a.q.row + head * a.q.head;
-    const T *const gb = (const T *)x.g.d_out.p + s.q0 * x.g.d_out.row + head * x.g.d_out.head;
-    const float *const lse_of = a.lse + (int64_t)head * a.nq + s.q0;
-    const float *const delta_of = x.delta + (int64_t)head * a.nq + s.q0;
-    const Bias by{(FEAT & kBias) && a.table ? bias : nullptr,
-                  (FEAT & kBias) && a.slopes ? -a.slopes[head] * bias_unit(a, FEAT & kCap) : 0.0f, a.reach};
-    if constexpr (FEAT & kBias) {
-      if (a.table) {
-        __syncthreads();
-        load_bias<T>(a, head, bias_unit(a, FEAT & kCap), bias, tid, THREADS);
-      }
-    }
-    auto fetch = [&](int t) {
-      const int left = s.nq - t * BQ;
-      qt.get(qb + (int64_t)(t * BQ) * a.q.row, a.q.row, left, tid);
-      gt.get(gb + (int64_t)(t * BQ) * x.g.d_out.row, x.g.d_out.row, left, tid);
-      // a row that sees nothing has lse -inf
-      tags.get((const int32_t *)lse_of + t * BQ, left, tid);
-      if (tid < BQ) {
-        const int r = min(t * BQ + tid, s.nq - 1);
-        lse = lse_of[r];
-        delta = delta_of[r];
-        if (a.q_docs) qdoc = a.q_docs[s.q0 + r];
-      }
-    };
-    if (t_first < t_end) fetch(t_first);
-    for (int t = t_first, tn; t < t_end; t = tn, buf ^= 1) {
-      char *const ql = smem + buf * 2 * QO::BYTES, *const gl = ql + QO::BYTES;
+  // A step's rows on their way: in registers while the step before it is
+  // computed.
+  struct {
+    QO q, g;
+    typename QO::Tags tags;
+    float lse, delta;
+    int doc;
+  } e;
+  auto fetch = [&](int g, int t) {
+    const int head = kvh * x.group + g, left = s.nq - t * BQ;
+    const int64_t row = s.q0 + t * BQ;
+    e.q.get((const T *)a.q.p + row * a.q.row + head * a.q.head, a.q.row, left, tid);
+    e.g.get((const T *)x.g.d_out.p + row * x.g.d_out.row + head * x.g.d_out.head, x.g.d_out.row, left, tid);
+    const int64_t at = (int64_t)head * a.nq + row;
+    // a row that sees nothing has lse -inf
+    e.tags.get((const int32_t *)a.lse + at, left, tid);
+    const int r = min(tid, left - 1);
+    e.lse = a.lse[at + r];
+    e.delta = x.delta[at + r];
+    e.doc = (a.q_docs ? a.q_docs + row : (const int32_t *)a.lse + at)[r];
+  };
+  auto put = [&](int t, int buf) {
+    // such rows, and those past the last, are cleared: P is 0 at -inf
+    char *const ql = smem + buf * 2 * QO::BYTES;
+    const int left = s.nq - t * BQ;
+    if (tid < BQ) {
       float *const st = stat + buf * 2 * BQ;
-      {
-        // such rows, and those past the last, are cleared: P is 0 at +inf
-        if (tid < BQ) {
-          const bool there = lse > -INFINITY && t * BQ + tid < s.nq;
-          st[tid] = there ? lse * kLog2e : INFINITY;
-          st[BQ + tid] = there ? delta : 0.0f;
-          qdocs[buf * BQ + tid] = qdoc < 0 ? -2 : qdoc;
-        }
-        auto keep = [&](int l) { return __builtin_bit_cast(float, l) > -INFINITY; };
-        qt.put(ql, s.nq - t * BQ, a.dim, tid, false, tags, keep);
-        gt.put(gl, s.nq - t * BQ, a.dim, tid, false, tags, keep);
-      }
-      __syncthreads();
-      tn = next(t + 1);
-      if (tn < t_end) fetch(tn);
-      const int p0 = t * BQ + s.shift;  // place of the step's first query
-      if (p0 > hi_max || p0 + BQ <= lo_min) continue;
-      const bool masked = a.q_docs || p0 < lo_max || p0 + BQ - 1 > hi_min;
-      unsigned bits = ~0u;
-      if (masked) {
-        bits = row_bits(p0, lo, hi, h);
-        if (a.q_docs && !docs.tile(qdocs + buf * BQ, lane, &bits)) continue;
-      }
+      const bool there = e.lse > -INFINITY && tid < left;
+      st[tid] = there ? sc.c2 - e.lse * kLog2e : -INFINITY;
+      st[BQ + tid] = there ? e.delta : 0.0f;
+      if (a.q_docs) qdocs[buf * BQ + tid] = e.doc < 0 ? -2 : e.doc;
+    }
+    auto keep = [&](int l) { return __builtin_bit_cast(float, l) > -INFINITY; };
+    e.q.put(ql, left, a.dim, tid, false, e.tags, keep);
+    e.g.put(ql + QO::BYTES, left, a.dim, tid, false, e.tags, keep);
+  };
+  e.q.init(a.q.row, a.dim, tid);
+  e.g.init(x.g.d_out.row, a.dim, tid);
 
-      v16f z = v16f{}, dp = v16f{}, bz = v16f{};
-      if constexpr (FEAT & kBias) bz = by.template at<-1>(key - p0 - 4 * h, k_lo - p0 - 31, k_hi - p0);
-      if constexpr (FEAT == kBias) z = bz;
+  auto compute = [&](int g, int t, int buf) {
+    const int r0 = 32 * qw, p0 = t * BQ + r0 + s.shift;  // the wave's first row, its place
+    if (p0 > hi_max || p0 + 32 <= lo_min) return;
+    const bool masked = a.q_docs || p0 < lo_max || p0 + 31 > hi_min;
+    unsigned bits = ~0u;
+    if (masked) {
+      bits = row_bits(p0, lo, hi, h);
+      if (a.q_docs && !docs.tile(qdocs + buf * BQ + r0, lane, &bits)) return;
+    }
+    const char *const ql = smem + buf * 2 * QO::BYTES, *const gl = ql + QO::BYTES;
+    const float *const st = stat + buf * 2 * BQ + r0;
+    v16f z = v16f{}, dp = v16f{}, bz = v16f{};
+    if constexpr (FEAT & kBias) {
+      const Bias by{a.table ? bias + (g & 1) * attend_bias_len(a.reach) : nullptr,
+                    a.slopes ? -a.slopes[kvh * x.group + g] * bias_unit(a, FEAT & kCap) : 0.0f, a.reach};
+      bz = by.template at<-1>(key - p0 - 4 * h, k_lo - p0 - 31, k_hi - p0);
+    }
+    if constexpr (FEAT == kBias) z = bz;
 #pragma unroll
-      for (int i = 0; i < KS; i++) {
-        z = mfma16(QO::rows(ql, 0, i, lane), k[i], z);
-        dp = mfma16(QO::rows(gl, 0, i, lane), v[i], dp);
+    for (int i = 0; i < KS; i++)
+      if (within<T>(16 * i, a.dim)) {
+        z = mfma16(QO::rows(ql, r0, i, lane), k[i], z);
+        dp = mfma16(QO::rows(gl, r0, i, lane), v[i], dp);
       }
-      float by_cap[16];
-      shape_scores<T, FEAT>(z, by_cap, sc, bz);
-      float pr[16];
+    float by_cap[16], pr[16], ds[16];
+    const float gain = shape_scores<T, FEAT>(z, by_cap, sc, bz);
 #pragma unroll
-      for (int g4 = 0; g4 < 4; g4++) {
-        const f4 l = *(const f4 *)(st + 8 * g4 + 4 * h);
+    for (int g4 = 0; g4 < 4; g4++) {
+      const f4 less = *(const f4 *)(st + 8 * g4 + 4 * h);
 #pragma unroll
-        for (int e = 0; e < 4; e++) pr[4 * g4 + e] = exp2_fast(z[4 * g4 + e] - l[e]);
-      }
-      if (masked) {
+      for (int e = 0; e < 4; e++) pr[4 * g4 + e] = exp2_fast(__builtin_fmaf(z[4 * g4 + e], gain, less[e]));
+    }
+    if (masked) {
 #pragma unroll
-        for (int r = 0; r < 16; r++) pr[r] = if_bit(bits, r, pr[r]);
-      }
-      float ds[16];
+      for (int r = 0; r < 16; r++) pr[r] = if_bit(bits, r, pr[r]);
+    }
 #pragma unroll
-      for (int g4 = 0; g4 < 4; g4++) {
-        const f4 dl = *(const f4 *)(st + BQ + 8 * g4 + 4 * h);
+    for (int g4 = 0; g4 < 4; g4++) {
+      const f4 dl = *(const f4 *)(st + BQ + 8 * g4 + 4 * h);
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
-          const int r = 4 * g4 + e;
-          ds[r] = pr[r] * (dp[r] - dl[e]);
-          if constexpr (FEAT & kCap) ds[r] *= by_cap[r];
-        }
-      }
-      // P and dS are rounded to the rows' type, as dO and Q are
-#pragma unroll
-      for (int w = 0; w < 2; w++) {
-        const Frag pf = pack8<Frag>(pr + 8 * w), sf = pack8<Frag>(ds + 8 * w);
-#pragma unroll
-        for (int d = 0; d < ND; d++) {
-          dv[d] = mfma16(QO::cols(gl, 16 * w, d, lane), pf, dv[d]);
-          dk[d] = mfma16(QO::cols(ql, 16 * w, d, lane), sf, dk[d]);
-        }
+      for (int e = 0; e < 4; e++) {
+        const int r = 4 * g4 + e;
+        ds[r] = pr[r] * (dp[r] - dl[e]);
+        if constexpr (FEAT & kCap) ds[r] *= by_cap[r];
       }
     }
+    // P and dS are rounded to the rows' type, as dO and Q are
+#pragma unroll
+    for (int w = 0; w < 2; w++) {
+      const Frag pf = pack8<Frag>(pr + 8 * w), sf = pack8<Frag>(ds + 8 * w);
+#pragma unroll
+      for (int d = 0; d < ND; d++) {
+        if (!within<T>(32 * d, a.dim)) continue;
+        dv[d] = mfma16(QO::cols(gl, r0 + 16 * w, d, lane), pf, dv[d]);
+        dk[d] = mfma16(QO::cols(ql, r0 + 16 * w, d, lane), sf, dk[d]);
+      }
+    }
+  };
+
+  // The steps of every head that shares the keys, one after another.
+  auto bias_of = [&](int g) {
+    if constexpr (FEAT & kBias)
+      if (a.table)
+        load_bias<T>(a, kvh * x.group + g, bias_unit(a, FEAT & kCap), bias + (g & 1) * attend_bias_len(a.reach), tid,
+                     THREADS);
+  };
+  const bool any = t_first < t_end;
+  if (any) {
+    fetch(0, t_first);
+    bias_of(0);
+    put(t_first, 0);
+  }
+  for (int g = 0, t = t_first, buf = 0; any && g < x.group; buf ^= 1) {
+    int then_g = g, then = next(t + 1);
+    if (then >= t_end) then_g++, then = t_first;
+    const bool more = then_g < x.group;
+    __syncthreads();
+    if (more) fetch(then_g, then);
+    compute(g, t, buf);
+    if (more) {
+      if (then_g != g) bias_of(then_g);
+      put(then, buf ^ 1);
+    }
+    g = then_g, t = then;
+  }
+  if constexpr (Sh::SHARE == 2) {
+    // the second wave's sums, through LDS to the first: dK's, then dV's
+    static_assert(4 * QO::BYTES >= 2 * 64 * 16 * ND * 4, "");
+    f4 *const sums = (f4 *)smem + kw * 64 * 4 * ND + lane;
+    auto meet = [&](v16f *acc) {
+      __syncthreads();
+      if (qw == 1)
+#pragma unroll
+        for (int d = 0; d < ND; d++)
+#pragma unroll
+          for (int g = 0; g < 4; g++)
+            sums[64 * (4 * d + g)] = f4{acc[d][4 * g], acc[d][4 * g + 1], acc[d][4 * g + 2], acc[d][4 * g + 3]};
+      __syncthreads();
+      if (qw == 0)
+#pragma unroll
+        for (int d = 0; d < ND; d++)
+#pragma unroll
+          for (int g = 0; g < 4; g++) {
+            const f4 v = sums[64 * (4 * d + g)];
+#pragma unroll
+            for (int e = 0; e < 4; e++) acc[d][4 * g + e] += v[e];
+          }
+    };
+    meet(dk);
+    meet(dv);
   }
   auto to = [&](const ixh_heads &t) {
     return [&, t](int i) {
-      const int r = first + wave * 32 + i;
-      return r < s.nk ? (T *)t.p + (int64_t)(s.k0 + r) * t.row + kvh * t.head : (T *)nullptr;
+      const int r = first + kw * 32 + i;
+      return qw == 0 && r < s.nk ? (T *)t.p + (int64_t)(s.k0 + r) * t.row + kvh * t.head : (T *)nullptr;
     };
   };
   char *const mine_lds = smem + wave * (32 * DT * (int)sizeof(T));
@@ -546,7 +598,7 @@ bool run_dq(const AttendArgs &x, hipStream_t s) {
 template <class T, int DT, int FEAT>
 bool run_dkv(const AttendArgs &x, hipStream_t s) {
   typedef DkvShape<T, DT> Sh;
-  const int shm = Sh::BIAS + ((FEAT & kBias) && x.a.table ? 4 * attend_bias_len(x.a.reach) : 0);
+  const int shm = Sh::BIAS + ((FEAT & kBias) && x.a.table ? 2 * 4 * attend_bias_len(x.a.reach) : 0);
   static PerDevice lds;
   if (!lds_granted(lds, (const void *)attend_dkv_kernel<T, DT, FEAT>, 160 << 10)) return false;
   attend_dkv_kernel<T, DT, FEAT><<<dim3((unsigned)(x.slots * x.a.kv_heads)), Sh::THREADS, shm, s>>>(x);

@@ -288,42 +288,69 @@ __device__ __forceinline__ void store_rows(const v16f *acc, float f, char *lds, 
   }
 }
 
+// Whether a step of the products at this column is taken: a float32 one costs
+// 8 slow MFMAs, so those past `dim` are left out; for 16-bit types the branch
+// costs more than the MFMA.
+template <class T>
+__device__ __forceinline__ bool within(int column, int dim) {
+  return sizeof(T) == 2 || column < dim;
+}
+
 // ---- sequences and masks ----------------------------------------------------
 
 // offs[i] as a row of an array of n rows, whatever it holds.
 __device__ __forceinline__ int row_at(const int32_t *offs, int i, int n) { return min(max(offs[i], 0), n); }
 
-// The sequence of a slot (attend_slots) and its block of rows: a search by
-// the whole wave, 64 sequences a step.
-__device__ __forceinline__ void find_block(const int32_t *offs, int B, int n, int rows, int pack, int64_t slot, int *seq,
-                                           int64_t *block) {
-  const int lane = __lane_id();
-  int lo = 0, count = B;
-  while (count > 1) {
-    const int step = (count + 63) / 64;
-    const int b = lo + lane * step;
-    const bool mine = lane * step < count && (int64_t)row_at(offs, b, n) * pack / rows + b <= slot;
-    const int at = max(0, __popcll(__ballot(mine)) - 1);
-    lo += at * step;
-    count = min(step, count - at * step);
-  }
-  lo = __builtin_amdgcn_readfirstlane(lo);
-  *seq = lo;
-  *block = slot - ((int64_t)row_at(offs, lo, n) * pack / rows + lo);
-}
-
 // One sequence: its rows in the packed arrays.
 struct Seq {
   int q0, nq, k0, nk, shift, prefix;  // shift: a query's place among the keys less its row
-  __device__ __forceinline__ Seq(const ixh_attend_args &a, int b) {
-    q0 = row_at(a.q_offs, b, a.nq);
-    nq = max(row_at(a.q_offs, b + 1, a.nq) - q0, 0);
-    k0 = row_at(a.k_offs, b, a.nk);
-    nk = max(row_at(a.k_offs, b + 1, a.nk) - k0, 0);
-    shift = nk - nq;
-    prefix = a.prefix ? a.prefix[b] : 0;
-  }
 };
+
+// The sequence of a slot (attend_slots) of `offs` (a's q_offs or k_offs) and
+// its block of rows: a search by the whole wave, 256 sequences a step, each
+// lane with four places side by side, and the ends of the sequence found come
+// out of the last step's values.
+__device__ __forceinline__ Seq find_block(const ixh_attend_args &a, bool by_keys, int rows, int pack, int64_t slot,
+                                          int64_t *block) {
+  const int32_t *const offs = by_keys ? a.k_offs : a.q_offs;
+  const int n = by_keys ? a.nk : a.nq, lane = __lane_id();
+  int lo = 0, count = a.B, at, v[5];
+  for (;;) {
+    const int step = (count + 255) / 256;
+#pragma unroll
+    for (int e = 0; e < 5; e++) v[e] = row_at(offs, min(lo + (4 * lane + e) * step, a.B), n);
+    int hits = 0;
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      const int i = (4 * lane + e) * step;
+      hits += __popcll(__ballot(i < count && (int64_t)v[e] * pack / rows + lo + i <= slot));
+    }
+    at = __builtin_amdgcn_readfirstlane(max(hits - 1, 0));
+    if (step == 1) break;
+    lo += at * step;
+    count = min(step, count - at * step);
+  }
+  const int b = lo + at;
+  const int from = at & 3;
+  const int x = from == 0 ? v[0] : from == 1 ? v[1] : from == 2 ? v[2] : v[3];
+  const int y = from == 0 ? v[1] : from == 1 ? v[2] : from == 2 ? v[3] : v[4];
+  const int first = __builtin_amdgcn_readlane(x, at >> 2), end = __builtin_amdgcn_readlane(y, at >> 2);
+  *block = slot - ((int64_t)first * pack / rows + b);
+  int first2 = first, end2 = end;
+  if (a.q_offs != a.k_offs) {
+    const int32_t *const others = by_keys ? a.q_offs : a.k_offs;
+    first2 = row_at(others, b, by_keys ? a.nq : a.nk);
+    end2 = row_at(others, b + 1, by_keys ? a.nq : a.nk);
+  }
+  Seq s;
+  s.q0 = by_keys ? first2 : first;
+  s.k0 = by_keys ? first : first2;
+  s.nq = max((by_keys ? end2 : end) - s.q0, 0);
+  s.nk = max((by_keys ? end : end2) - s.k0, 0);
+  s.shift = s.nk - s.nq;
+  s.prefix = a.prefix ? a.prefix[b] : 0;
+  return s;
+}
 
 // The keys lo..hi that the query at place p sees (documents apart); empty
 // where hi < lo. Both ends grow with p.
@@ -370,21 +397,44 @@ __device__ __forceinline__ void doc_steps(const int32_t *mine, int first, int la
     mn = min(mn, __shfl_xor(mn, o));
     mx = max(mx, __shfl_xor(mx, o));
   }
+  // A wave takes the 64 steps of a word, 16 at a time: 4 lanes a step, each
+  // with every 4th row of it, whose loads are launched together.
   for (int w = wave; w < kDocWords && t0 + 64 * w < t1; w += WAVES) {
-    const int t = t0 + 64 * w + lane;
-    int tmn = INT32_MAX, tmx = -1;
-    if (t < t1) {
+    uint64_t word = 0;
+    for (int part = 0; part < 4 && t0 + 64 * w + 16 * part < t1; part++) {
+      const int t = t0 + 64 * w + 16 * part + (lane >> 2);
+      int d[STEP / 4];
 #pragma unroll
-      for (int i = 0; i < STEP; i++) {
-        const int d = theirs[min(t * STEP + i, n - 1)];
-        tmn = min(tmn, d < 0 ? INT32_MAX : d);
-        tmx = max(tmx, d);
+      for (int i = 0; i < STEP / 4; i++) d[i] = theirs[min(t * STEP + 4 * i + (lane & 3), n - 1)];
+#pragma unroll
+      for (int i = 0; i < STEP / 4; i++) asm volatile("" : "+v"(d[i]));  // none is used before all are on their way
+      int tmn = INT32_MAX, tmx = -1;
+#pragma unroll
+      for (int i = 0; i < STEP / 4; i++) {
+        tmn = min(tmn, d[i] < 0 ? INT32_MAX : d[i]);
+        tmx = max(tmx, d[i]);
       }
+#pragma unroll
+      for (int o = 1; o < 4; o <<= 1) {
+        tmn = min(tmn, __shfl_xor(tmn, o));
+        tmx = max(tmx, __shfl_xor(tmx, o));
+      }
+      uint64_t hit = __ballot(t < t1 && tmx >= 0 && mx >= 0 && tmn <= mx && tmx >= mn);
+      // every 4th lane's bit, side by side
+      hit &= 0x1111111111111111ull;
+      hit = (hit | hit >> 3) & 0x0303030303030303ull;
+      hit = (hit | hit >> 6) & 0x000f000f000f000full;
+      hit = (hit | hit >> 12) & 0x000000ff000000ffull;
+      hit = (hit | hit >> 24) & 0xffffull;
+      word |= hit << (16 * part);
     }
-    const uint64_t lv = __ballot(tmx >= 0 && mx >= 0 && tmn <= mx && tmx >= mn);
-    if (lane == 0) live[w] = lv;
+    if (lane == 0) live[w] = word;
   }
 }
+// Every load so far has come in: a loop's own loads need no wait for those
+// of values that it only reads.
+__device__ __forceinline__ void loads_done() { __builtin_amdgcn_s_waitcnt(0x0f70); }
+
 // The first live step from t on, t1 if none.
 __device__ __forceinline__ int next_live(const uint64_t *live, int t, int t0, int t1) {
   while (t < t1) {

@@ -42,10 +42,8 @@ void attend_fwd_kernel(AttendArgs x) {
   // last blocks first: under a causal mask they have the most keys
   const int pack = x.pack, nh = pack > 1 ? a.kv_heads : a.heads;
   const int hb = blockIdx.x % nh;
-  int b;
   int64_t blk;
-  find_block(a.q_offs, a.B, a.nq, ROWS, pack, x.slots - 1 - blockIdx.x / nh, &b, &blk);
-  const Seq s(a, b);
+  const Seq s = find_block(a, false, ROWS, pack, x.slots - 1 - blockIdx.x / nh, &blk);
   const int64_t rows = (int64_t)s.nq * pack;
   if (blk * ROWS >= rows) return;
   const int kvh = pack > 1 ? hb : hb / x.group;
@@ -80,19 +78,6 @@ void attend_fwd_kernel(AttendArgs x) {
     }
   }
 
-  const ColumnDocs docs(a.q_docs ? a.q_docs[s.q0 + tok] : 0);
-  if (a.q_docs)
-    doc_steps<BK, WAVES>(a.q_docs + s.q0, (int)(blk * ROWS / pack), (int)((min(blk * ROWS + ROWS, rows) - 1) / pack),
-                         a.k_docs + s.k0, s.nk, t_begin, t_end, live, wave, lane);
-  if constexpr (FEAT & kBias) {
-    if (a.table)
-      for (int i = 0; i < pack; i++)
-        load_bias<T>(a, pack > 1 ? hb * pack + i : hb, bias_unit(a, FEAT & kCap), bias + i * attend_bias_len(a.reach), tid, THREADS);
-  }
-  if (a.q_docs || (FEAT & kBias)) __syncthreads();
-
-  auto next = [&](int t) { return a.q_docs ? next_live(live, t, t_begin, t_end) : t; };
-
   // Q's fragments, columns past dim 0
   Frag q[KS];
   {
@@ -102,16 +87,6 @@ void attend_fwd_kernel(AttendArgs x) {
   }
   const T *const kb = (const T *)a.k.p + s.k0 * a.k.row + kvh * a.k.head;
   const T *const vb = (const T *)a.v.p + s.k0 * a.v.row + kvh * a.v.head;
-  const Score sc(a, FEAT & kCap);
-  const Bias by{(FEAT & kBias) && a.table ? bias + sub * attend_bias_len(a.reach) : nullptr,
-                (FEAT & kBias) && a.slopes ? -a.slopes[head] * bias_unit(a, FEAT & kCap) : 0.0f, a.reach};
-
-  v16f acc[ND];
-#pragma unroll
-  for (int d = 0; d < ND; d++) acc[d] = v16f{};
-  // the maximum so far; what scores are taken against
-  float m = -INFINITY, ref = 0.0f, sum = 0.0f;
-
   KV kt, vt;
   typename KV::Tags tags;
   kt.init(a.k.row, a.dim, tid);
@@ -126,6 +101,33 @@ void attend_fwd_kernel(AttendArgs x) {
       if (tid < BK) kdoc = a.k_docs[s.k0 + t * BK + min(tid, left - 1)];
     }
   };
+
+  // the first step's keys are on their way while the documents and the bias
+  // are looked at (documents may skip that step)
+  if (!a.q_docs && t_begin < t_end) fetch(t_begin);
+
+  const ColumnDocs docs(a.q_docs ? a.q_docs[s.q0 + tok] : 0);
+  if (a.q_docs)
+    doc_steps<BK, WAVES>(a.q_docs + s.q0, (int)(blk * ROWS / pack), (int)((min(blk * ROWS + ROWS, rows) - 1) / pack),
+                         a.k_docs + s.k0, s.nk, t_begin, t_end, live, wave, lane);
+  if constexpr (FEAT & kBias) {
+    if (a.table)
+      for (int i = 0; i < pack; i++)
+        load_bias<T>(a, pack > 1 ? hb * pack + i : hb, bias_unit(a, FEAT & kCap), bias + i * attend_bias_len(a.reach), tid, THREADS);
+  }
+  if (a.q_docs || (FEAT & kBias)) __syncthreads();
+
+  auto next = [&](int t) { return a.q_docs ? next_live(live, t, t_begin, t_end) : t; };
+
+  const Score sc(a, FEAT & kCap);
+  const Bias by{(FEAT & kBias) && a.table ? bias + sub * attend_bias_len(a.reach) : nullptr,
+                (FEAT & kBias) && a.slopes ? -a.slopes[head] * bias_unit(a, FEAT & kCap) : 0.0f, a.reach};
+
+  v16f acc[ND];
+#pragma unroll
+  for (int d = 0; d < ND; d++) acc[d] = v16f{};
+  // the maximum so far; what scores are taken against
+  float m = -INFINITY, ref = 0.0f, sum = 0.0f;
 
   // The 32 keys from key j0 of the sequence, row r0 of the step in LDS:
   // scores, running maximum and sum, and their part of the output.
@@ -142,7 +144,8 @@ void attend_fwd_kernel(AttendArgs x) {
     float gain = sc.c1;
     if constexpr (FEAT == kBias) z = by.template at<1>(d0, near, far);
 #pragma unroll
-    for (int i = 0; i < KS; i++) z = mfma16(KV::rows(kl, r0, i, lane), q[i], z);
+    for (int i = 0; i < KS; i++)
+      if (within<T>(16 * i, a.dim)) z = mfma16(KV::rows(kl, r0, i, lane), q[i], z);
     if constexpr (FEAT & kCap) {
 #pragma unroll
       for (int r = 0; r < 16; r++) z[r] = capped<T>(sc, z[r]);
@@ -202,13 +205,14 @@ void attend_fwd_kernel(AttendArgs x) {
     for (int v = 0; v < 2; v++) {
       const Frag pf = pack8<Frag>(pr + 8 * v);
 #pragma unroll
-      for (int d = 0; d < ND; d++) acc[d] = mfma16(KV::cols(vl, r0 + 16 * v, d, lane), pf, acc[d]);
+      for (int d = 0; d < ND; d++)
+        if (within<T>(32 * d, a.dim)) acc[d] = mfma16(KV::cols(vl, r0 + 16 * v, d, lane), pf, acc[d]);
     }
   };
 
   int buf = 0;
   int t = next(t_begin);
-  if (t < t_end) fetch(t);
+  if (a.q_docs && t < t_end) fetch(t);
   while (t < t_end) {
     char *const kl = smem + buf * 2 * KV::BYTES, *const vl = kl + KV::BYTES;
     {
@@ -271,10 +275,12 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs x) {
   if (row >= row_at(a.q_offs, a.B, a.nq) || row < row_at(a.q_offs, 0, a.nq)) return;
   float m = -INFINITY;
   const int64_t step = (int64_t)a.nq * a.heads;
+#pragma unroll 8
   for (int i = 0; i < x.splits; i++) m = __builtin_fmaxf(m, x.part_ml[2 * (i * step + rh)]);
   const float ref = m == -INFINITY ? 0.0f : m;
   f4 o{};
   float sum = 0.0f;
+#pragma unroll 8
   for (int i = 0; i < x.splits; i++) {
     const float f = exp2_fast(x.part_ml[2 * (i * step + rh)] - ref);
     sum = __builtin_fmaf(f, x.part_ml[2 * (i * step + rh) + 1], sum);
