@@ -76,13 +76,32 @@ def _out(op, name, t, like):
     return t, _heads(op, name, t, like, like.shape)
 
 
+_WORKSPACE = struct.Struct("@Pq")  # the argument structs' last two
+
+
 def _call(f, like, *args):
     device = like.get_device()
-    _lib.check(f(device, *args, torch.cuda.current_stream(device).cuda_stream))
+    _lib.check(f(device, *args, _stream(device)))
 
 
-def _space(like, n):
-    return torch.empty(n, dtype=torch.uint8, device=like.device) if n else None
+def _stream(device):
+    """The address of torch's current stream of the GPU."""
+    return torch.cuda.current_stream(device).cuda_stream
+
+
+# the same without the object around it, where this torch has it
+_stream = getattr(torch._C, "_cuda_getCurrentRawStream", _stream)
+
+
+def _with_space(packed, like, size, *more):
+    """The packed arguments with the workspace that `size` asks for, and the
+    workspace: held until the call has queued its work."""
+    n = C.c_int64()
+    _lib.check(size(packed, *more, C.byref(n)))
+    if n.value == 0:
+        return packed, None
+    space = like.new_empty(n.value, dtype=torch.uint8)
+    return packed[:-_WORKSPACE.size] + _WORKSPACE.pack(space.data_ptr(), n.value), space
 
 
 def _attend_args(op, q, k, v, offs, k_offs, scale, cap, slopes, table, buckets, docs, k_docs, causal, prefix, window):
@@ -114,19 +133,6 @@ def _attend_args(op, q, k, v, offs, k_offs, scale, cap, slopes, table, buckets, 
         -1 if window is None else window)
 
 
-def _with_space(args, q, backward):
-    """The packed arguments with their workspace, and the workspace: held
-    until the call has queued its work."""
-    n = C.c_int64()
-    L = _lib.lib()
-    packed = _ATTEND.pack(*args, 0, 0)
-    _lib.check(L.ixh_attend_workspace(packed, backward, C.byref(n)))
-    if n.value == 0:
-        return packed, None
-    space = _space(q, n.value)
-    return _ATTEND.pack(*args, space.data_ptr(), n.value), space
-
-
 def attend(q, k, v, offs, k_offs=None, *, scale=None, cap=0.0, slopes=None, table=None, buckets=None, docs=None,
            k_docs=None, causal=False, prefix=None, window=-1, out=None, want_lse=False):
     """softmax(scores) v over each query's visible keys: [rows][heads][dim],
@@ -147,9 +153,11 @@ def attend(q, k, v, offs, k_offs=None, *, scale=None, cap=0.0, slopes=None, tabl
     before, after = _attend_args(op, q, k, v, offs, k_offs, scale, cap, slopes, table, buckets, docs, k_docs, causal,
                                  prefix, window)
     out, place = _out(op, "out", out, q)
-    lse = torch.empty((q.shape[1], q.shape[0]), dtype=torch.float32, device=q.device) if want_lse else None
-    args, space = _with_space((*before, *place, *after, lse.data_ptr() if want_lse else 0), q, 0)
-    _call(_lib.lib().ixh_attend, q, args)
+    lse = q.new_empty((q.shape[1], q.shape[0]), dtype=torch.float32) if want_lse else None
+    L = _lib.lib()
+    args, space = _with_space(_ATTEND.pack(*before, *place, *after, lse.data_ptr() if want_lse else 0, 0, 0), q,
+                              L.ixh_attend_workspace, 0)
+    _call(L.ixh_attend, q, args)
     return (out, lse) if want_lse else out
 
 
@@ -168,8 +176,9 @@ def attend_backward(d_out, q, k, v, out, lse, offs, k_offs=None, *, scale=None, 
     place = _heads(op, "out", out, q, q.shape)
     (dq, dq_at), (dk, dk_at), (dv, dv_at) = _out(op, "dq", dq, q), _out(op, "dk", dk, k), _out(op, "dv", dv, v)
     dtable = torch.empty_like(table) if table is not None else None
-    args, space = _with_space((*before, *place, *after, lse_at), q, 1)
-    _call(_lib.lib().ixh_attend_backward, q, args,
+    L = _lib.lib()
+    args, space = _with_space(_ATTEND.pack(*before, *place, *after, lse_at, 0, 0), q, L.ixh_attend_workspace, 1)
+    _call(L.ixh_attend_backward, q, args,
           _GRADS.pack(*given, *dq_at, *dk_at, *dv_at, dtable.data_ptr() if dtable is not None else 0))
     return dq, dk, dv, dtable
 
@@ -236,13 +245,11 @@ def qk_norm_rope_backward(dq_out, dk_out, q, k, cos=None, sin=None, *, pos=None,
     dq_gamma = None if q_gamma is None else torch.empty_like(q_gamma)
     dk_gamma = None if k_gamma is None else torch.empty_like(k_gamma)
     none = (0, 0, 0)
-    args, space = (*before, *none, *none, *after), None
+    L = _lib.lib()
+    args, space = _NORM_ROPE.pack(*before, *none, *none, *after, 0, 0), None
     if dq_gamma is not None or dk_gamma is not None:
-        n = C.c_int64()
-        _lib.check(_lib.lib().ixh_qk_norm_rope_workspace(_NORM_ROPE.pack(*args, 0, 0), C.byref(n)))
-        space = _space(q, n.value)  # held until the call has queued its work
-    _call(_lib.lib().ixh_qk_norm_rope_backward, q,
-          _NORM_ROPE.pack(*args, space.data_ptr() if space is not None else 0, n.value if space is not None else 0),
+        args, space = _with_space(args, q, L.ixh_qk_norm_rope_workspace)
+    _call(L.ixh_qk_norm_rope_backward, q, args,
           _NORM_ROPE_GRADS.pack(*given, *dq_at, *dk_at, dq_gamma.data_ptr() if dq_gamma is not None else 0,
                                 dk_gamma.data_ptr() if dk_gamma is not None else 0))
     return dq, dk, dq_gamma, dk_gamma

@@ -129,7 +129,7 @@ Plan plan_forward(AttendArgs &x) {
   x.group = a.heads / a.kv_heads;
   x.pack = 1;
   const int64_t B = std::max(a.B, 1);
-  if (x.group > 1 && (int64_t)a.nq * x.group <= 32 * B &&
+  if (x.group > 1 && (int64_t)a.nq * x.group <= std::min<int64_t>(32 * B, INT32_MAX) &&
       (!a.table || 4LL * x.group * attend_bias_len(a.reach) <= 32 << 10))
     x.pack = x.group;
   p.few = (int64_t)a.nq * x.pack <= 48 * B;
@@ -156,7 +156,7 @@ int64_t plan_backward(AttendArgs &x) {
   x.dist_parts = 0;
   if (a.table) {
     const int64_t span = 2LL * a.reach + 1;
-    x.dist_parts = (int)std::min<int64_t>(kMaxDistParts, x.slots / 16 + 1);
+    x.dist_parts = kMaxDistParts;
     bytes += up(4 * x.slots * a.heads * span) + up(4 * x.dist_parts * a.heads * span);
   }
   return bytes;
@@ -247,6 +247,10 @@ int ixh_attend_backward(int device, const ixh_attend_args *a, const ixh_attend_g
     w += up(4LL * a->heads * a->nq);
     x.dist = (float *)w;
     x.dist_sum = (float *)(w + up(4 * x.slots * a->heads * span));
+    if (x.slots <= kMaxDistParts) {  // few enough for the last kernel alone
+      x.dist_sum = x.dist;
+      x.dist_parts = (int)x.slots;
+    }
   }
   if (a->B > 0) {
     if (!launch_attend_dq(x, st)) return fail(IXH_EHIP, "linalg: hip: AttendBackward: LDS refused");
@@ -256,7 +260,7 @@ int ixh_attend_backward(int device, const ixh_attend_args *a, const ixh_attend_g
     if (!launch_attend_dkv(y, st)) return fail(IXH_EHIP, "linalg: hip: AttendBackward: LDS refused");
     if ((rc = launched("attend_dkv"))) return rc;
   } else {
-    x.slots = 0;
+    x.slots = x.dist_parts = 0;
   }
   if (g->dtable) {
     launch_attend_dtable(x, st);

@@ -16,7 +16,8 @@ namespace ixh {
 namespace {
 
 // 16 products to scores: a score is then z * gain + c2 (Score's) in base 2.
-// Under a cap slope_of gets its derivative by the product, in units of scale.
+// Under a cap slope_of gets a quarter of its derivative by the product, in
+// units of scale (u - u^2): the 4 comes with the scale, after the sums.
 template <class T, int FEAT>
 __device__ __forceinline__ float shape_scores(v16f &z, float *slope_of, const Score &sc, const v16f &bias) {
   if constexpr (!(FEAT & kCap)) return sc.c1;
@@ -25,7 +26,7 @@ __device__ __forceinline__ float shape_scores(v16f &z, float *slope_of, const Sc
   for (int r = 0; r < 16; r++) {
     const float u = capped<T>(sc, z[r]);
     z[r] = FEAT & kBias ? __builtin_fmaf(u, gain, bias[r]) : u;
-    slope_of[r] = 4.0f * u * (1.0f - u);
+    slope_of[r] = __builtin_fmaf(-u, u, u);
   }
   return FEAT & kBias ? 1.0f : gain;
 }
@@ -251,7 +252,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : DT == 64 ? 3 : 2) void at
     }
   }
 
-  store_rows<T, DT>(acc, a.scale, smem + wave * (32 * DT * (int)sizeof(T)), a.dim, lane, [&](int i) {
+  store_rows<T, DT>(acc, (FEAT & kCap ? 4.0f : 1.0f) * a.scale, smem + wave * (32 * DT * (int)sizeof(T)), a.dim, lane, [&](int i) {
     const int r = first + wave * 32 + i;
     return r < s.nq ? (T *)x.g.dq.p + (int64_t)(s.q0 + r) * x.g.dq.row + head * x.g.dq.head : (T *)nullptr;
   });
@@ -528,7 +529,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 || DT == 128 ? 1 : 2) void atte
     };
   };
   char *const mine_lds = smem + wave * (32 * DT * (int)sizeof(T));
-  store_rows<T, DT>(dk, a.scale, mine_lds, a.dim, lane, to(x.g.dk));
+  store_rows<T, DT>(dk, (FEAT & kCap ? 4.0f : 1.0f) * a.scale, mine_lds, a.dim, lane, to(x.g.dk));
   store_rows<T, DT>(dv, 1.0f, mine_lds, a.dim, lane, to(x.g.dv));
 }
 
@@ -631,7 +632,7 @@ bool launch_attend_dkv(const AttendArgs &x, hipStream_t s) { return by_type(x, f
 
 void launch_attend_dtable(const AttendArgs &x, hipStream_t s) {
   const int span = 2 * x.a.reach + 1;
-  attend_dist_kernel<<<dim3((span + 63) / 64, x.a.heads, x.dist_parts), 256, 0, s>>>(x);
+  if (x.dist_sum != x.dist) attend_dist_kernel<<<dim3((span + 63) / 64, x.a.heads, x.dist_parts), 256, 0, s>>>(x);
   const int shm = 8 * span;
   switch (x.a.type) {
     case IXH_TYPE_F32: attend_dtable_kernel<float><<<x.a.heads, 256, shm, s>>>(x); break;

@@ -309,7 +309,7 @@ struct Seq {
 // The sequence of a slot (attend_slots) of `offs` (a's q_offs or k_offs) and
 // its block of rows: a search by the whole wave, 256 sequences a step, each
 // lane with four places side by side, and the ends of the sequence found come
-// out of the last step's values.
+// out of the last step's values. n * pack is below 2^31.
 __device__ __forceinline__ Seq find_block(const ixh_attend_args &a, bool by_keys, int rows, int pack, int64_t slot,
                                           int64_t *block) {
   const int32_t *const offs = by_keys ? a.k_offs : a.q_offs;
@@ -323,7 +323,7 @@ __device__ __forceinline__ Seq find_block(const ixh_attend_args &a, bool by_keys
 #pragma unroll
     for (int e = 0; e < 4; e++) {
       const int i = (4 * lane + e) * step;
-      hits += __popcll(__ballot(i < count && (int64_t)v[e] * pack / rows + lo + i <= slot));
+      hits += __popcll(__ballot(i < count && (unsigned)(v[e] * pack) / (unsigned)rows + lo + i <= slot));
     }
     at = __builtin_amdgcn_readfirstlane(max(hits - 1, 0));
     if (step == 1) break;
@@ -335,7 +335,7 @@ __device__ __forceinline__ Seq find_block(const ixh_attend_args &a, bool by_keys
   const int x = from == 0 ? v[0] : from == 1 ? v[1] : from == 2 ? v[2] : v[3];
   const int y = from == 0 ? v[1] : from == 1 ? v[2] : from == 2 ? v[3] : v[4];
   const int first = __builtin_amdgcn_readlane(x, at >> 2), end = __builtin_amdgcn_readlane(y, at >> 2);
-  *block = slot - ((int64_t)first * pack / rows + b);
+  *block = slot - ((unsigned)(first * pack) / (unsigned)rows + b);
   int first2 = first, end2 = end;
   if (a.q_offs != a.k_offs) {
     const int32_t *const others = by_keys ? a.q_offs : a.k_offs;

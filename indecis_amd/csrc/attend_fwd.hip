@@ -44,14 +44,15 @@ void attend_fwd_kernel(AttendArgs x) {
   const int hb = blockIdx.x % nh;
   int64_t blk;
   const Seq s = find_block(a, false, ROWS, pack, x.slots - 1 - blockIdx.x / nh, &blk);
-  const int64_t rows = (int64_t)s.nq * pack;
+  const int rows = s.nq * pack;
   if (blk * ROWS >= rows) return;
+  const int row0 = (int)blk * ROWS, row1 = min(row0 + ROWS, rows);
   const int kvh = pack > 1 ? hb : hb / x.group;
 
-  // the lane's query: row, head, place; rows past the last repeat it
-  const int64_t r = min(blk * ROWS + wave * 32 + (lane & 31), rows - 1);
-  const bool mine = blk * ROWS + wave * 32 + (lane & 31) < rows;
-  const int tok = pack > 1 ? (int)((unsigned)r / (unsigned)pack) : (int)r, sub = pack > 1 ? (int)(r - (int64_t)tok * pack) : 0;
+  // the lane's query: its row, head and place; rows past the last repeat it
+  auto token = [&](int r) { return pack > 1 ? r / pack : r; };
+  const int r = min(row0 + wave * 32 + (lane & 31), rows - 1), tok = token(r), sub = r - tok * pack;
+  const bool mine = row0 + wave * 32 + (lane & 31) < rows;
   const int head = pack > 1 ? hb * pack + sub : hb;
   const int p = tok + s.shift;
   int lo, hi;
@@ -60,15 +61,14 @@ void attend_fwd_kernel(AttendArgs x) {
   const int lo_min = __builtin_amdgcn_readlane(lo, 0), lo_max = __builtin_amdgcn_readlane(lo, 31);
   const int hi_min = __builtin_amdgcn_readlane(hi, 0);
   // a wave past the last row has nothing to see
-  const int hi_max = blk * ROWS + wave * 32 < rows ? __builtin_amdgcn_readlane(hi, 31) : -1;
+  const int hi_max = row0 + wave * 32 < rows ? __builtin_amdgcn_readlane(hi, 31) : -1;
 
   // the workgroup's steps of keys
   int t_begin, t_end;
   {
     int l, u, unused;
-    const int64_t last = min(blk * ROWS + ROWS, rows) - 1;
-    key_bounds(a, s, (int)(blk * ROWS / pack) + s.shift, &l, &unused);
-    key_bounds(a, s, (int)(last / pack) + s.shift, &unused, &u);
+    key_bounds(a, s, token(row0) + s.shift, &l, &unused);
+    key_bounds(a, s, token(row1 - 1) + s.shift, &unused, &u);
     t_begin = l / BK;
     t_end = u >= l ? u / BK + 1 : t_begin;
     if (x.splits > 1) {
@@ -102,14 +102,10 @@ void attend_fwd_kernel(AttendArgs x) {
     }
   };
 
-  // the first step's keys are on their way while the documents and the bias
-  // are looked at (documents may skip that step)
-  if (!a.q_docs && t_begin < t_end) fetch(t_begin);
-
   const ColumnDocs docs(a.q_docs ? a.q_docs[s.q0 + tok] : 0);
   if (a.q_docs)
-    doc_steps<BK, WAVES>(a.q_docs + s.q0, (int)(blk * ROWS / pack), (int)((min(blk * ROWS + ROWS, rows) - 1) / pack),
-                         a.k_docs + s.k0, s.nk, t_begin, t_end, live, wave, lane);
+    doc_steps<BK, WAVES>(a.q_docs + s.q0, token(row0), token(row1 - 1), a.k_docs + s.k0, s.nk, t_begin, t_end, live, wave,
+                         lane);
   if constexpr (FEAT & kBias) {
     if (a.table)
       for (int i = 0; i < pack; i++)
@@ -212,7 +208,7 @@ void attend_fwd_kernel(AttendArgs x) {
 
   int buf = 0;
   int t = next(t_begin);
-  if (a.q_docs && t < t_end) fetch(t);
+  if (t < t_end) fetch(t);
   while (t < t_end) {
     char *const kl = smem + buf * 2 * KV::BYTES, *const vl = kl + KV::BYTES;
     {
@@ -255,10 +251,9 @@ void attend_fwd_kernel(AttendArgs x) {
   }
   if (a.lse && mine && h == 0) a.lse[(int64_t)head * a.nq + row] = (ref + __builtin_amdgcn_logf(sum)) * kLn2;
   store_rows<T, DT>(acc, sum > 0.0f ? 1.0f / sum : 0.0f, smem + wave * (32 * DT * (int)sizeof(T)), a.dim, lane, [&](int i) {
-    const int64_t r = blk * ROWS + wave * 32 + i;
+    const int r = row0 + wave * 32 + i, tok = token(r);
     if (r >= rows) return (T *)nullptr;
-    const int tok = pack > 1 ? (int)((unsigned)r / (unsigned)pack) : (int)r;
-    return (T *)a.o.p + (s.q0 + tok) * a.o.row + (pack > 1 ? hb * pack + (int)(r - (int64_t)tok * pack) : hb) * a.o.head;
+    return (T *)a.o.p + (s.q0 + tok) * a.o.row + (pack > 1 ? hb * pack + r - tok * pack : hb) * a.o.head;
   });
 }
 
