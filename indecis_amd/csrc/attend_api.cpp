@@ -147,17 +147,19 @@ Plan plan_forward(AttendArgs &x) {
   return p;
 }
 
-int64_t plan_backward(AttendArgs &x) {
+// The dQ kernel's slots in x; the dK, dV kernel's in *key_slots.
+int64_t plan_backward(AttendArgs &x, int64_t *key_slots) {
   const ixh_attend_args &a = x.a;
   x.group = a.heads / a.kv_heads;
   x.pack = 1;
   x.slots = attend_slots(a.nq, a.B, 128, 1);
+  *key_slots = attend_slots(a.nk, a.B, attend_dkv_keys(type_size(a.type), a.dim), 1);
   int64_t bytes = up(4LL * a.heads * a.nq);
   x.dist_parts = 0;
   if (a.table) {
     const int64_t span = 2LL * a.reach + 1;
     x.dist_parts = kMaxDistParts;
-    bytes += up(4 * x.slots * a.heads * span) + up(4 * x.dist_parts * a.heads * span);
+    bytes += up(4 * *key_slots * a.heads * span) + up(4 * x.dist_parts * a.heads * span);
   }
   return bytes;
 }
@@ -185,7 +187,8 @@ int ixh_attend_workspace(const ixh_attend_args *a, int backward, int64_t *bytes)
   AttendArgs x{};
   x.a = *a;
   fill_in(x.a);
-  *bytes = backward ? plan_backward(x) : plan_forward(x).work;
+  int64_t key_slots;
+  *bytes = backward ? plan_backward(x, &key_slots) : plan_forward(x).work;
   return IXH_OK;
 }
 
@@ -232,8 +235,8 @@ int ixh_attend_backward(int device, const ixh_attend_args *a, const ixh_attend_g
         (rc = check_heads("AttendBackward", "dv", g->dv, a->type)))
       return rc;
   }
-  const int64_t need = plan_backward(x);
-  const int64_t key_slots = attend_slots(a->nk, a->B, attend_dkv_keys(type_size(a->type), a->dim), 1);
+  int64_t key_slots;
+  const int64_t need = plan_backward(x, &key_slots);
   if (x.slots * a->heads > kMaxGrid || key_slots * a->kv_heads > kMaxGrid)
     return fail(IXH_EINVAL, "linalg: AttendBackward: too many rows and heads for one launch");
   if ((rc = check_workspace("AttendBackward", a->workspace, a->workspace_bytes, need))) return rc;
@@ -242,28 +245,28 @@ int ixh_attend_backward(int device, const ixh_attend_args *a, const ixh_attend_g
   hipStream_t const st = (hipStream_t)stream;
   char *w = (char *)a->workspace;
   x.delta = (float *)w;
+  AttendArgs y = x;
+  y.slots = key_slots;
   if (g->dtable) {
     const int64_t span = 2LL * a->reach + 1;
     w += up(4LL * a->heads * a->nq);
-    x.dist = (float *)w;
-    x.dist_sum = (float *)(w + up(4 * x.slots * a->heads * span));
-    if (x.slots <= kMaxDistParts) {  // few enough for the last kernel alone
-      x.dist_sum = x.dist;
-      x.dist_parts = (int)x.slots;
+    y.dist = (float *)w;
+    y.dist_sum = (float *)(w + up(4 * key_slots * a->heads * span));
+    if (key_slots <= kMaxDistParts) {  // few enough for the last kernel alone
+      y.dist_sum = y.dist;
+      y.dist_parts = (int)key_slots;
     }
   }
   if (a->B > 0) {
     if (!launch_attend_dq(x, st)) return fail(IXH_EHIP, "linalg: hip: AttendBackward: LDS refused");
     if ((rc = launched("attend_dq"))) return rc;
-    AttendArgs y = x;
-    y.slots = key_slots;
     if (!launch_attend_dkv(y, st)) return fail(IXH_EHIP, "linalg: hip: AttendBackward: LDS refused");
     if ((rc = launched("attend_dkv"))) return rc;
   } else {
-    x.slots = x.dist_parts = 0;
+    y.slots = y.dist_parts = 0;
   }
   if (g->dtable) {
-    launch_attend_dtable(x, st);
+    launch_attend_dtable(y, st);
     return launched("attend_dtable");
   }
   return IXH_OK;

@@ -6,9 +6,16 @@
 //   dQ = scale dS K, dK = scale dS^T Q, dV = P^T dO.
 // Two kernels, so that no sum crosses workgroups and no result depends on
 // an order of atomics: one has a block of queries and runs over the keys
-// (dQ, delta and the bias' sums), one has a block of keys and runs over
-// the queries of every head that shares them (dK, dV). Both take S and dP
-// again: 7 products for the 5 of one kernel with atomics.
+// (dQ), one has a block of keys and runs over the queries of every head that
+// shares them (dK, dV and the bias' sums). Both take S and dP again: 7
+// products for the 5 of one kernel with atomics.
+//
+// Precision of 16-bit rows. delta from the rounded o is off by the rounding
+// times |dO|, which every dZ of the row inherits. The first kernel's sum of
+// a row's dZ is minus that error (the exact ones add up to 0), so it passes
+// the second a delta that is right to 32 bits. dQ itself is taken from dS in
+// two pieces, rounded and what that took off: an eighth product, in place of
+// an error as large as the result's own rounding.
 #include "attend_device.h"
 #include "ixh_internal.h"
 
@@ -54,21 +61,11 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : DT == 64 ? 3 : 2) void at
   int *const kdocs = (int *)(smem + Sh::DOCS);
   uint64_t *const live = (uint64_t *)(smem + Sh::LIVE);
   float *const bias = (float *)(smem + Sh::BIAS);
-  // sums of dZ by distance, an array each wave, with the bias' ends
-  const int span = 2 * a.reach + 1, len = attend_bias_len(a.reach);
-  float *const dist = bias + len;
-
   const int head = blockIdx.x % a.heads, kvh = head / x.group;
   const int64_t slot = x.slots - 1 - blockIdx.x / a.heads;
   int64_t blk;
   const Seq s = find_block(a, false, ROWS, 1, slot, &blk);
-  const bool grad_table = (FEAT & kBias) && x.dist;
-  float *const dist_out = grad_table ? x.dist + (slot * a.heads + head) * span : nullptr;
-  if (blk * ROWS >= s.nq) {
-    if (grad_table)
-      for (int i = tid; i < span; i += THREADS) dist_out[i] = 0.0f;
-    return;
-  }
+  if (blk * ROWS >= s.nq) return;
   const int first = (int)(blk * ROWS);
   const int tok = min(first + wave * 32 + (lane & 31), s.nq - 1);
   const bool mine = first + wave * 32 + (lane & 31) < s.nq;
@@ -111,7 +108,6 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : DT == 64 ? 3 : 2) void at
       for (int e = 0; e < 8; e++) delta = __builtin_fmaf(frag_at(dO[i], e), frag_at(o, e), delta);
     }
     delta = half_sum(delta);
-    if (mine && h == 0) x.delta[(int64_t)head * a.nq + row] = delta;
   }
   const T *const kb = (const T *)a.k.p + s.k0 * a.k.row + kvh * a.k.head;
   const T *const vb = (const T *)a.v.p + s.k0 * a.v.row + kvh * a.v.head;
@@ -122,16 +118,13 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : DT == 64 ? 3 : 2) void at
                 (FEAT & kBias) && a.slopes ? -a.slopes[head] * unit : 0.0f, a.reach};
   if constexpr (FEAT & kBias) {
     if (a.table) load_bias<T>(a, head, unit, bias, tid, THREADS);
-    if (grad_table)
-      for (int i = tid; i < Sh::WAVES * len; i += THREADS) dist[i] = 0.0f;
   }
   if (a.q_docs)
     doc_steps<BK, Sh::WAVES>(a.q_docs + s.q0, first, min(first + ROWS, s.nq) - 1, a.k_docs + s.k0, s.nk, t_begin, t_end,
                              live, wave, lane);
   if (a.q_docs || (FEAT & kBias)) __syncthreads();
   auto next = [&](int t) { return a.q_docs ? next_live(live, t, t_begin, t_end) : t; };
-  float *const my_dist = dist + wave * len;
-  float below = 0.0f, above = 0.0f;  // dZ at distances of -reach and less, reach and more
+  float row_sum = 0.0f;  // of dZ
 
   v16f acc[ND];
 #pragma unroll
@@ -195,96 +188,40 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : DT == 64 ? 3 : 2) void at
 #pragma unroll
       for (int r = 0; r < 16; r++) dz[r] = if_bit(bits, r, dz[r]);
     }
-    if constexpr (FEAT & kBias) {
-      if (grad_table) {
-        if (!mine) {
 #pragma unroll
-          for (int r = 0; r < 16; r++) dz[r] = 0.0f;
-        }
-        if (flat) {
-          float part = 0.0f;
-#pragma unroll
-          for (int r = 0; r < 16; r++) part += dz[r];
-          if (near >= a.reach)
-            above += part;
-          else
-            below += part;
-        } else {
-          // Along the tile's diagonals: a row of 64 lanes moves one lane up
-          // for each key and takes up that key's 32 values, so that lane l
-          // ends with the sum at distance j0 - p + 31 - l (p: lane 0's).
-          // A swap with zeros gives both halves' keys as such rows. Two
-          // chains of 16 keys, for the adds' latency; the first, 16 lanes
-          // low, is brought up at the end.
-          float row[2] = {};
-#pragma unroll
-          for (int g = 0; g < 2; g++) {
-            float up[2][4], dn[2][4];
-#pragma unroll
-            for (int e = 0; e < 4; e++)
-#pragma unroll
-              for (int c = 0; c < 2; c++) halves_apart(dz[4 * (2 * c + g) + e], &up[c][e], &dn[c][e]);
-#pragma unroll
-            for (int e = 0; e < 4; e++)
-#pragma unroll
-              for (int c = 0; c < 2; c++) row[c] = lane_up(row[c]) + up[c][e];
-#pragma unroll
-            for (int e = 0; e < 4; e++)
-#pragma unroll
-              for (int c = 0; c < 2; c++) row[c] = lane_up(row[c]) + dn[c][e];
-          }
-          const float low = __shfl(row[0], lane - 16);
-          my_dist[j0 - p_lo + 31 - lane + a.reach + kBiasPad] += (lane >= 16 ? low : 0.0f) + row[1];
-        }
-      }
-    }
+    for (int r = 0; r < 16; r++) row_sum += dz[r];
     if constexpr (FEAT & kCap) {
 #pragma unroll
       for (int r = 0; r < 16; r++) dz[r] *= by_cap[r];
     }
-    // dS is rounded to the rows' type, as K is; scale comes after the sum
+    // dS in the rows' type, as K is, and what that rounding took off; scale
+    // comes after the sum
 #pragma unroll
     for (int v = 0; v < 2; v++) {
       const Frag f = pack8<Frag>(dz + 8 * v);
+      Frag rest{};
+      if constexpr (sizeof(T) == 2) {
+        float off[8];
+#pragma unroll
+        for (int e = 0; e < 8; e++) off[e] = dz[8 * v + e] - frag_at(f, e);
+        rest = pack8<Frag>(off);
+      }
 #pragma unroll
       for (int d = 0; d < ND; d++)
-        if (within<T>(32 * d, a.dim)) acc[d] = mfma16(KV::cols(kl, 16 * v, d, lane), f, acc[d]);
+        if (within<T>(32 * d, a.dim)) {
+          const Frag k = KV::cols(kl, 16 * v, d, lane);
+          acc[d] = mfma16(k, f, acc[d]);
+          if constexpr (sizeof(T) == 2) acc[d] = mfma16(k, rest, acc[d]);
+        }
     }
   }
 
+  row_sum = half_sum(row_sum);
+  if (mine && h == 0) x.delta[(int64_t)head * a.nq + row] = delta + row_sum;
   store_rows<T, DT>(acc, (FEAT & kCap ? 4.0f : 1.0f) * a.scale, smem + wave * (32 * DT * (int)sizeof(T)), a.dim, lane, [&](int i) {
     const int r = first + wave * 32 + i;
     return r < s.nq ? (T *)x.g.dq.p + (int64_t)(s.q0 + r) * x.g.dq.row + head * x.g.dq.head : (T *)nullptr;
   });
-  if constexpr (FEAT & kBias) {
-    if (grad_table) {
-      // the ends: the lanes' sums in a fixed order, then the arrays past the
-      // reach, which are the ends' too
-#pragma unroll
-      for (int o = 1; o < 64; o <<= 1) {
-        above += __shfl_xor(above, o);
-        below += __shfl_xor(below, o);
-      }
-      float *const d = dist + wave * len;
-      if (lane == 0) d[0] += below, d[len - 1] += above;
-      __syncthreads();
-      for (int i = tid; i < len; i += THREADS) {
-        float v = 0.0f;
-#pragma unroll
-        for (int w = 0; w < Sh::WAVES; w++) v += dist[w * len + i];
-        dist[i] = v;
-      }
-      __syncthreads();
-      for (int i = tid; i < span; i += THREADS) {
-        float v = dist[i + kBiasPad];
-        if (i == 0)
-          for (int e = 0; e < kBiasPad; e++) v += dist[e];
-        if (i == span - 1)
-          for (int e = 1; e <= kBiasPad; e++) v += dist[i + kBiasPad + e];
-        dist_out[i] = v;
-      }
-    }
-  }
 }
 
 // ---- dK, dV -----------------------------------------------------------------
@@ -321,12 +258,23 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 || DT == 128 ? 1 : 2) void atte
   float *const stat = (float *)(smem + Sh::STAT);
   int *const qdocs = (int *)(smem + Sh::DOCS);
   uint64_t *const live = (uint64_t *)(smem + Sh::LIVE);
+  // the bias of two heads in turn; the sums of dZ by distance, an array each
+  // wave, with the bias' ends
   float *const bias = (float *)(smem + Sh::BIAS);
+  const int span = 2 * a.reach + 1, len = attend_bias_len(a.reach);
+  float *const dist = bias + 2 * len, *const my_dist = dist + wave * len;
+  const bool grad_table = (FEAT & kBias) && x.dist;
 
   const int kvh = blockIdx.x % a.kv_heads;
   int64_t blk;
   const Seq s = find_block(a, true, KEYS, 1, blockIdx.x / a.kv_heads, &blk);
-  if (blk * KEYS >= s.nk) return;
+  const int64_t slot = blockIdx.x / a.kv_heads;
+  if (blk * KEYS >= s.nk) {
+    if (grad_table)
+      for (int g = 0; g < x.group; g++)
+        for (int i = tid; i < span; i += THREADS) x.dist[(slot * a.heads + kvh * x.group + g) * span + i] = 0.0f;
+    return;
+  }
   const int first = (int)(blk * KEYS);
   const int key = min(first + kw * 32 + (lane & 31), s.nk - 1);
   int lo, hi;  // places of the queries that see the key
@@ -334,6 +282,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 || DT == 128 ? 1 : 2) void atte
   const int k_lo = __builtin_amdgcn_readlane(key, 0), k_hi = __builtin_amdgcn_readlane(key, 31);
   const int lo_min = __builtin_amdgcn_readlane(lo, 0), lo_max = __builtin_amdgcn_readlane(lo, 31);
   const int hi_min = __builtin_amdgcn_readlane(hi, 0);
+  const bool mine = first + kw * 32 + (lane & 31) < s.nk;
   const int hi_max = first + kw * 32 < s.nk ? __builtin_amdgcn_readlane(hi, 31) : INT32_MIN;
   int t_begin, t_end;  // steps of BQ queries
   {
@@ -411,6 +360,39 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 || DT == 128 ? 1 : 2) void atte
   e.q.init(a.q.row, a.dim, tid);
   e.g.init(x.g.d_out.row, a.dim, tid);
 
+  float below = 0.0f, above = 0.0f;  // dZ at distances of -reach and less, reach and more
+  auto clear_dist = [&] {
+    for (int i = lane; i < len; i += 64) my_dist[i] = 0.0f;
+    below = above = 0.0f;
+  };
+  // A head's sums: the ends' lanes in a fixed order, the waves' arrays, and
+  // what lies past the reach, which is the ends' too.
+  auto write_dist = [&](int g) {
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      above += __shfl_xor(above, o);
+      below += __shfl_xor(below, o);
+    }
+    if (lane == 0) my_dist[0] += below, my_dist[len - 1] += above;
+    __syncthreads();
+    for (int i = tid; i < len; i += THREADS) {
+      float v = 0.0f;
+#pragma unroll
+      for (int w = 0; w < Sh::WAVES; w++) v += dist[w * len + i];
+      dist[i] = v;
+    }
+    __syncthreads();
+    float *const out = x.dist + (slot * a.heads + kvh * x.group + g) * span;
+    for (int i = tid; i < span; i += THREADS) {
+      float v = dist[i + kBiasPad];
+      if (i == 0)
+        for (int e = 0; e < kBiasPad; e++) v += dist[e];
+      if (i == span - 1)
+        for (int e = 1; e <= kBiasPad; e++) v += dist[i + kBiasPad + e];
+      out[i] = v;
+    }
+    __syncthreads();
+  };
   auto compute = [&](int g, int t, int buf) {
     const int r0 = 32 * qw, p0 = t * BQ + r0 + s.shift;  // the wave's first row, its place
     if (p0 > hi_max || p0 + 32 <= lo_min) return;
@@ -424,7 +406,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 || DT == 128 ? 1 : 2) void atte
     const float *const st = stat + buf * 2 * BQ + r0;
     v16f z = v16f{}, dp = v16f{}, bz = v16f{};
     if constexpr (FEAT & kBias) {
-      const Bias by{a.table ? bias + (g & 1) * attend_bias_len(a.reach) : nullptr,
+      const Bias by{a.table ? bias + (g & 1) * len : nullptr,
                     a.slopes ? -a.slopes[kvh * x.group + g] * bias_unit(a, FEAT & kCap) : 0.0f, a.reach};
       bz = by.template at<-1>(key - p0 - 4 * h, k_lo - p0 - 31, k_hi - p0);
     }
@@ -454,8 +436,55 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 || DT == 128 ? 1 : 2) void atte
       for (int e = 0; e < 4; e++) {
         const int r = 4 * g4 + e;
         ds[r] = pr[r] * (dp[r] - dl[e]);
-        if constexpr (FEAT & kCap) ds[r] *= by_cap[r];
       }
+    }
+    if constexpr (FEAT & kBias) {
+      if (grad_table) {
+        float dz[16];
+#pragma unroll
+        for (int r = 0; r < 16; r++) dz[r] = mine ? ds[r] : 0.0f;
+        const int near = k_lo - p0 - 31, far = k_hi - p0;
+        if (near >= a.reach || far <= -a.reach) {
+          float part = 0.0f;
+#pragma unroll
+          for (int r = 0; r < 16; r++) part += dz[r];
+          if (near >= a.reach)
+            above += part;
+          else
+            below += part;
+        } else {
+          // Along the tile's diagonals: a row of 64 lanes moves one lane up
+          // for each query and takes up that query's 32 values, so that
+          // lane l ends with the sum at distance k_lo - p0 - 31 + l. A swap
+          // with zeros gives both halves' queries as such rows. Two chains
+          // of 16 queries, for the adds' latency; the first, 16 lanes low,
+          // is brought up at the end. (LDS adds by distance took 128 cycles
+          // an instruction: 302 -> 86 us over 48 sequences of 64-512.)
+          float row[2] = {};
+#pragma unroll
+          for (int g = 0; g < 2; g++) {
+            float up[2][4], dn[2][4];
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+#pragma unroll
+              for (int c = 0; c < 2; c++) halves_apart(dz[4 * (2 * c + g) + e], &up[c][e], &dn[c][e]);
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+#pragma unroll
+              for (int c = 0; c < 2; c++) row[c] = lane_up(row[c]) + up[c][e];
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+#pragma unroll
+              for (int c = 0; c < 2; c++) row[c] = lane_up(row[c]) + dn[c][e];
+          }
+          const float low = __shfl(row[0], lane - 16);
+          my_dist[near + lane + a.reach + kBiasPad] += (lane >= 16 ? low : 0.0f) + row[1];
+        }
+      }
+    }
+    if constexpr (FEAT & kCap) {
+#pragma unroll
+      for (int r = 0; r < 16; r++) ds[r] *= by_cap[r];
     }
     // P and dS are rounded to the rows' type, as dO and Q are
 #pragma unroll
@@ -474,10 +503,16 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 || DT == 128 ? 1 : 2) void atte
   auto bias_of = [&](int g) {
     if constexpr (FEAT & kBias)
       if (a.table)
-        load_bias<T>(a, kvh * x.group + g, bias_unit(a, FEAT & kCap), bias + (g & 1) * attend_bias_len(a.reach), tid,
+        load_bias<T>(a, kvh * x.group + g, bias_unit(a, FEAT & kCap), bias + (g & 1) * len, tid,
                      THREADS);
   };
   const bool any = t_first < t_end;
+  if constexpr (FEAT & kBias)
+    if (grad_table) {
+      clear_dist();
+      if (!any)
+        for (int g = 0; g < x.group; g++) write_dist(g);
+    }
   if (any) {
     fetch(0, t_first);
     bias_of(0);
@@ -490,6 +525,11 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 || DT == 128 ? 1 : 2) void atte
     __syncthreads();
     if (more) fetch(then_g, then);
     compute(g, t, buf);
+    if constexpr (FEAT & kBias)
+      if (grad_table && then_g != g) {
+        write_dist(g);
+        clear_dist();
+      }
     if (more) {
       if (then_g != g) bias_of(then_g);
       put(then, buf ^ 1);
@@ -535,7 +575,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 || DT == 128 ? 1 : 2) void atte
 
 // ---- the table's gradient ----------------------------------------------------
 
-// Sums of dZ by distance over the workgroups of attend_dq_kernel: a part of
+// Sums of dZ by distance over the workgroups of attend_dkv_kernel: a part of
 // them each block, four strands a distance.
 __global__ __launch_bounds__(256) void attend_dist_kernel(AttendArgs x) {
   __shared__ float strand[4][64];
@@ -590,7 +630,7 @@ template <class T, int DT, int FEAT>
 bool run_dq(const AttendArgs &x, hipStream_t s) {
   typedef DqShape<T, DT> Sh;
   const int len = (FEAT & kBias) && x.a.table ? attend_bias_len(x.a.reach) : 0;
-  const int shm = Sh::BIAS + 4 * len * (1 + Sh::WAVES);
+  const int shm = Sh::BIAS + 4 * len;
   static PerDevice lds;
   if (!lds_granted(lds, (const void *)attend_dq_kernel<T, DT, FEAT>, 160 << 10)) return false;
   attend_dq_kernel<T, DT, FEAT><<<dim3((unsigned)(x.slots * x.a.heads)), Sh::THREADS, shm, s>>>(x);
@@ -599,7 +639,8 @@ bool run_dq(const AttendArgs &x, hipStream_t s) {
 template <class T, int DT, int FEAT>
 bool run_dkv(const AttendArgs &x, hipStream_t s) {
   typedef DkvShape<T, DT> Sh;
-  const int shm = Sh::BIAS + ((FEAT & kBias) && x.a.table ? 2 * 4 * attend_bias_len(x.a.reach) : 0);
+  const int len = (FEAT & kBias) && x.a.table ? attend_bias_len(x.a.reach) : 0;
+  const int shm = Sh::BIAS + 4 * len * (2 + Sh::WAVES);
   static PerDevice lds;
   if (!lds_granted(lds, (const void *)attend_dkv_kernel<T, DT, FEAT>, 160 << 10)) return false;
   attend_dkv_kernel<T, DT, FEAT><<<dim3((unsigned)(x.slots * x.a.kv_heads)), Sh::THREADS, shm, s>>>(x);
