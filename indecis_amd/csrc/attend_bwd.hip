@@ -22,20 +22,18 @@
 namespace ixh {
 namespace {
 
-// 16 products to scores: a score is then z * gain + c2 (Score's) in base 2.
-// Under a cap slope_of gets a quarter of its derivative by the product, in
-// units of scale (u - u^2): the 4 comes with the scale, after the sums.
+// 16 products to scores: z * the returned gain in base 2. Under a cap slope_of
+// gets their derivative by the product, in units of scale.
 template <class T, int FEAT>
 __device__ __forceinline__ float shape_scores(v16f &z, float *slope_of, const Score &sc, const v16f &bias) {
-  if constexpr (!(FEAT & kCap)) return sc.c1;
-  const float gain = cap_gain(sc);
+  if constexpr (!(FEAT & kCap)) return sc.gain;
+  tanh_tile<T>(z, sc);
 #pragma unroll
   for (int r = 0; r < 16; r++) {
-    const float u = capped<T>(sc, z[r]);
-    z[r] = FEAT & kBias ? __builtin_fmaf(u, gain, bias[r]) : u;
-    slope_of[r] = __builtin_fmaf(-u, u, u);
+    slope_of[r] = __builtin_fmaf(-z[r], z[r], 1.0f);
+    if constexpr (FEAT & kBias) z[r] = __builtin_fmaf(z[r], sc.gain, bias[r]);
   }
-  return FEAT & kBias ? 1.0f : gain;
+  return FEAT & kBias ? 1.0f : sc.gain;
 }
 
 // ---- dQ ---------------------------------------------------------------------
@@ -112,7 +110,6 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : DT == 64 ? 3 : 2) void at
   const T *const kb = (const T *)a.k.p + s.k0 * a.k.row + kvh * a.k.head;
   const T *const vb = (const T *)a.v.p + s.k0 * a.v.row + kvh * a.v.head;
   const Score sc(a, FEAT & kCap);
-  const float less = sc.c2 - lse2;
   const float unit = bias_unit(a, FEAT & kCap);
   const Bias by{(FEAT & kBias) && a.table ? bias : nullptr,
                 (FEAT & kBias) && a.slopes ? -a.slopes[head] * unit : 0.0f, a.reach};
@@ -125,6 +122,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : DT == 64 ? 3 : 2) void at
   if (a.q_docs || (FEAT & kBias)) __syncthreads();
   auto next = [&](int t) { return a.q_docs ? next_live(live, t, t_begin, t_end) : t; };
   float row_sum = 0.0f;  // of dZ
+  const bool one_step = t_end - t_begin == 1;
 
   v16f acc[ND];
 #pragma unroll
@@ -183,11 +181,20 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : DT == 64 ? 3 : 2) void at
     const float gain = shape_scores<T, FEAT>(z, by_cap, sc, bz);
     float dz[16];
 #pragma unroll
-    for (int r = 0; r < 16; r++) dz[r] = exp2_fast(__builtin_fmaf(z[r], gain, less)) * (dp[r] - delta);
+    for (int r = 0; r < 16; r++) dz[r] = exp2_fast(__builtin_fmaf(z[r], gain, -lse2));
     if (masked) {
 #pragma unroll
       for (int r = 0; r < 16; r++) dz[r] = if_bit(bits, r, dz[r]);
     }
+    if (one_step) {
+      // all of a row's keys are here: delta without o's rounding
+      delta = 0.0f;
+#pragma unroll
+      for (int r = 0; r < 16; r++) delta = __builtin_fmaf(dz[r], dp[r], delta);
+      delta = half_sum(delta);
+    }
+#pragma unroll
+    for (int r = 0; r < 16; r++) dz[r] *= dp[r] - delta;
 #pragma unroll
     for (int r = 0; r < 16; r++) row_sum += dz[r];
     if constexpr (FEAT & kCap) {
@@ -218,7 +225,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : DT == 64 ? 3 : 2) void at
 
   row_sum = half_sum(row_sum);
   if (mine && h == 0) x.delta[(int64_t)head * a.nq + row] = delta + row_sum;
-  store_rows<T, DT>(acc, (FEAT & kCap ? 4.0f : 1.0f) * a.scale, smem + wave * (32 * DT * (int)sizeof(T)), a.dim, lane, [&](int i) {
+  store_rows<T, DT>(acc, a.scale, smem + wave * (32 * DT * (int)sizeof(T)), a.dim, lane, [&](int i) {
     const int r = first + wave * 32 + i;
     return r < s.nq ? (T *)x.g.dq.p + (int64_t)(s.q0 + r) * x.g.dq.row + head * x.g.dq.head : (T *)nullptr;
   });
@@ -349,7 +356,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 || DT == 128 ? 1 : 2) void atte
     if (tid < BQ) {
       float *const st = stat + buf * 2 * BQ;
       const bool there = e.lse > -INFINITY && tid < left;
-      st[tid] = there ? sc.c2 - e.lse * kLog2e : -INFINITY;
+      st[tid] = there ? e.lse * -kLog2e : -INFINITY;
       st[BQ + tid] = there ? e.delta : 0.0f;
       if (a.q_docs) qdocs[buf * BQ + tid] = e.doc < 0 ? -2 : e.doc;
     }
@@ -569,7 +576,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 || DT == 128 ? 1 : 2) void atte
     };
   };
   char *const mine_lds = smem + wave * (32 * DT * (int)sizeof(T));
-  store_rows<T, DT>(dk, (FEAT & kCap ? 4.0f : 1.0f) * a.scale, mine_lds, a.dim, lane, to(x.g.dk));
+  store_rows<T, DT>(dk, a.scale, mine_lds, a.dim, lane, to(x.g.dk));
   store_rows<T, DT>(dv, 1.0f, mine_lds, a.dim, lane, to(x.g.dv));
 }
 

@@ -491,32 +491,49 @@ struct ColumnDocs {
 // FEAT: 1 a tanh cap, 2 a bias by distance.
 enum { kCap = 1, kBias = 2 };
 
-// Constants of a call's scores in base 2: z = c1 * s, or, capped,
-// z = c2 tanh(s * scale / cap); the softmax is 2^(z - maximum).
+// A call's scores in base 2: z = gain * q.k, or, capped, gain * tanh(c1 q.k);
+// the softmax is 2^(z - maximum).
 struct Score {
-  float c1, c2;
+  float c1, gain;
   __device__ __forceinline__ explicit Score(const ixh_attend_args &a, bool cap) {
-    if (cap) {
-      c1 = a.scale / a.cap;
-      c2 = a.cap * kLog2e;
-    } else {
-      c1 = a.scale * kLog2e;
-      c2 = 0;
-    }
+    c1 = cap ? a.scale / a.cap : 1.0f;
+    gain = (cap ? a.cap : a.scale) * kLog2e;
   }
 };
 
-// A capped score, c2 tanh(s c1), as c2 + cap_gain() * capped(): with
-// tanh(x) = 1 - 2u, u = 1 / (1 + e^2x), by the hardware's exponential and
-// reciprocal, off by about 1e-7 of 1, which next to a 16-bit result is
-// nothing. float32 takes the library's tanh, u = (1 - tanh) / 2. The
-// derivative is 1 - tanh^2 = 4 u (1 - u).
+// tanh(c1 z) of a tile's 16 scores a lane. Where every score of the wave is
+// within half the cap, as most are, an odd polynomial: tanh(x) / x over x^2
+// in 0..1/4 (interpolated at Chebyshev's nodes, 2.7e-8 off), 2 * 2^-24 of
+// tanh with its roundings and no dearer than an exponential and a
+// reciprocal. Else 1 - 2 / (1 + e^2x) by those, off by up to 2^-21 of 1, next
+// to a 16-bit result nothing, and for float32 the library's tanh.
 template <class T>
-__device__ __forceinline__ float capped(const Score &sc, float s) {
-  if constexpr (sizeof(T) == 4) return 0.5f - 0.5f * tanhf(s * sc.c1);
-  return __builtin_amdgcn_rcpf(1.0f + exp2_fast(s * (sc.c1 * (2 * kLog2e))));
+__device__ __forceinline__ void tanh_tile(v16f &z, const Score &sc) {
+  float most = 0.0f;
+#pragma unroll
+  for (int r = 0; r < 16; r++) {
+    z[r] *= sc.c1;
+    most = __builtin_fmaxf(most, __builtin_fabsf(z[r]));
+  }
+  if (__ballot(!(most <= 0.5f)) == 0) {
+#pragma unroll
+    for (int r = 0; r < 16; r++) {
+      const float x = z[r], y = x * x;
+      float p = __builtin_fmaf(y, 0.017141319811344147f, -0.05298924073576927f);
+      p = __builtin_fmaf(p, y, 0.13324828445911407f);
+      p = __builtin_fmaf(p, y, -0.3333307206630707f);
+      z[r] = __builtin_fmaf(p * y, x, x);
+    }
+  } else {
+#pragma unroll
+    for (int r = 0; r < 16; r++) {
+      if constexpr (sizeof(T) == 4)
+        z[r] = tanhf(z[r]);
+      else
+        z[r] = __builtin_fmaf(-2.0f, __builtin_amdgcn_rcpf(1.0f + exp2_fast(z[r] * (2 * kLog2e))), 1.0f);
+    }
+  }
 }
-__device__ __forceinline__ float cap_gain(const Score &sc) { return -2.0f * sc.c2; }
 
 // The bias starts the first product's sum, in units of q.k (bias / scale), so
 // that it costs no operation of its own; under a cap it is added to z, in
@@ -574,21 +591,22 @@ __device__ __forceinline__ unsigned row_bits(int j0, int lo, int hi, int h) {
   const unsigned below = (unsigned)((1ull << l) - 1), upto = (unsigned)((1ull << u) - 1);
   return (upto & ~below) >> (4 * h);
 }
+// All ones where the bit of register r is set, else 0: one instruction, which
+// the compiler would make a test, a comparison and a select of.
+__device__ __forceinline__ unsigned bit_mask(unsigned bits, int r) {
+  unsigned m;
+  asm("v_bfe_i32 %0, %1, %2, 1" : "=v"(m) : "v"(bits), "n"(8 * (r >> 2) + (r & 3)));
+  return m;
+}
 // v where the bit of register r is set, else -inf.
 __device__ __forceinline__ float or_minus_inf(unsigned bits, int r, float v) {
-  const unsigned m = (unsigned)__builtin_amdgcn_sbfe((int)bits, 8 * (r >> 2) + (r & 3), 1);
+  const unsigned m = bit_mask(bits, r);
   return __builtin_bit_cast(float, (__builtin_bit_cast(unsigned, v) & m) | (0xff800000u & ~m));
 }
 // v where the bit of register r is set, else 0.
 __device__ __forceinline__ float if_bit(unsigned bits, int r, float v) {
-  const unsigned m = (unsigned)__builtin_amdgcn_sbfe((int)bits, 8 * (r >> 2) + (r & 3), 1);
-  return __builtin_bit_cast(float, __builtin_bit_cast(unsigned, v) & m);
+  return __builtin_bit_cast(float, __builtin_bit_cast(unsigned, v) & bit_mask(bits, r));
 }
 
-__device__ __forceinline__ float max3(float a, float b, float c) {
-  float d;
-  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(d) : "v"(a), "v"(b), "v"(c));
-  return d;
-}
 
 }  // namespace ixh

@@ -135,17 +135,14 @@ void attend_fwd_kernel(AttendArgs x) {
       if (kd && !docs.tile(kd + r0, lane, &bits)) return;
     }
     const int d0 = j0 + 4 * h - p, near = j0 - p_hi, far = j0 + 31 - p_lo;
-    // a score is z * gain + c2 in base 2
-    v16f z{};
-    float gain = sc.c1;
+    v16f z{};  // a score is z * gain in base 2
+    float gain = sc.gain;
     if constexpr (FEAT == kBias) z = by.template at<1>(d0, near, far);
 #pragma unroll
     for (int i = 0; i < KS; i++)
       if (within<T>(16 * i, a.dim)) z = mfma16(KV::rows(kl, r0, i, lane), q[i], z);
     if constexpr (FEAT & kCap) {
-#pragma unroll
-      for (int r = 0; r < 16; r++) z[r] = capped<T>(sc, z[r]);
-      gain = cap_gain(sc);
+      tanh_tile<T>(z, sc);
       if constexpr (FEAT & kBias) {
         const v16f b = by.template at<1>(d0, near, far);
 #pragma unroll
@@ -158,10 +155,9 @@ void attend_fwd_kernel(AttendArgs x) {
     // query's first need their own maximum or rescale the sums.
     float part, pr[16];
     auto probabilities = [&] {
-      const float less = sc.c2 - ref;
       part = 0.0f;
 #pragma unroll
-      for (int r = 0; r < 16; r++) pr[r] = exp2_fast(__builtin_fmaf(z[r], gain, less));
+      for (int r = 0; r < 16; r++) pr[r] = exp2_fast(__builtin_fmaf(z[r], gain, -ref));
       if (masked) {
 #pragma unroll
         for (int r = 0; r < 16; r++) pr[r] = if_bit(bits, r, pr[r]);
@@ -175,13 +171,13 @@ void attend_fwd_kernel(AttendArgs x) {
     if (again) {
       float top = -INFINITY, y[16];
 #pragma unroll
-      for (int r = 0; r < 16; r++) y[r] = __builtin_fmaf(z[r], gain, sc.c2);
+      for (int r = 0; r < 16; r++) y[r] = z[r] * gain;
       if (masked) {
 #pragma unroll
         for (int r = 0; r < 16; r++) y[r] = or_minus_inf(bits, r, y[r]);
       }
 #pragma unroll
-      for (int r = 0; r < 16; r += 2) top = max3(y[r], y[r + 1], top);
+      for (int r = 0; r < 16; r++) top = __builtin_fmaxf(top, y[r]);
       top = half_max(top);
       const float next_m = __builtin_fmaxf(m, top);
       const float f = m == -INFINITY ? 0.0f : exp2_fast(m - next_m);
