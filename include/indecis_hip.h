@@ -459,7 +459,10 @@ int ixh_attend_workspace(const ixh_attend_args *a, int backward, int64_t *bytes)
  * finite, as a product with probability 0 reads them. */
 int ixh_attend(int device, const ixh_attend_args *a, void *stream);
 /* The gradients of ixh_attend at the same arguments, o and lse as it left
- * them: dq, dk (over the heads that share it), dv, and the table's. */
+ * them: dq, dk (over the heads that share it), dv, and the table's. In
+ * float16 a score's gradient, P (dP - sum dO o), has to stay in the type's
+ * range, as a scaled loss keeps it. The workspace of a table's gradient grows
+ * with keys / 64 * heads * (2 reach + 1) * 4 bytes. */
 int ixh_attend_backward(int device, const ixh_attend_args *a, const ixh_attend_grads *g, void *stream);
 
 /* The buckets of a learned distance bias, map [2 max_distance + 1] for

@@ -109,7 +109,7 @@ def _attend_args(op, q, k, v, offs, k_offs, scale, cap, slopes, table, buckets, 
     qh, kh, vh = _heads(op, "q", q), _heads(op, "k", k, q), _heads(op, "v", v, q)
     nq, heads, dim = q.shape
     nk, kv_heads, k_dim = k.shape
-    _need(k.shape == v.shape and k_dim == dim, op, "q, k and v do not fit together")
+    _need(k.shape == v.shape and k_dim == dim and dim > 0, op, "q, k and v do not fit together")
     B = offs.numel() - 1
     _need(B >= 0, op, "offs is not [sequences + 1]")
     n_buckets = reach = 0

@@ -71,7 +71,7 @@ int check_heads(const char *op, const char *name, const ixh_heads &t, int type) 
 // Reach 1024 is 8 KB of table a head in LDS and 64 KB of sums in the dQ
 // kernel, beside 32 to 64 KB of keys.
 constexpr int kMaxReach = 1024, kMaxBuckets = 65536, kMaxRows = 1 << 30;
-constexpr int64_t kMaxGrid = (1LL << 31) - 1;
+constexpr int64_t kMaxGrid = (1LL << 24) - 1;  // workgroups: a launch has fewer than 2^32 threads along x
 constexpr int kCus = 256;
 constexpr int kMaxSplits = 64;
 constexpr int kMaxDistParts = 16;
@@ -327,6 +327,9 @@ int ixh_rel_buckets(int buckets, int max_distance, int bidirectional, int32_t *m
 
 namespace {
 
+// Lanes of a row of this dimension.
+int row_lanes(int dim) { return dim <= 32 ? 4 : dim <= 64 ? 8 : dim <= 128 ? 16 : 32; }
+
 int check_norm_rope(const ixh_norm_rope_args *a) {
   if (!a) return fail(IXH_EINVAL, "linalg: QKNormRope: no arguments");
   if (!type_ok(a->type)) return fail(IXH_EINVAL, "linalg: QKNormRope: type %d", a->type);
@@ -350,14 +353,13 @@ int check_norm_rope(const ixh_norm_rope_args *a) {
   if (a->rot > 0 && a->n > 0 && (!a->cos || !a->sin || a->rows < 1))
     return fail(IXH_EINVAL, "linalg: QKNormRope: a rotation needs cos and sin");
   if (a->n == 0) return IXH_OK;
+  if (a->n / (256 / row_lanes(a->dim)) >= kMaxGrid)
+    return fail(IXH_EINVAL, "linalg: QKNormRope: too many rows for one launch (%d of %d columns)", a->n, a->dim);
   int rc;
   if (a->q_heads > 0 && (rc = check_heads("QKNormRope", "q", a->q, a->type))) return rc;
   if (a->k_heads > 0 && (rc = check_heads("QKNormRope", "k", a->k, a->type))) return rc;
   return IXH_OK;
 }
-
-// Lanes of a row of this dimension.
-int row_lanes(int dim) { return dim <= 32 ? 4 : dim <= 64 ? 8 : dim <= 128 ? 16 : 32; }
 
 // Every row's heads to one group of lanes where there are rows enough to
 // fill the chip (it keeps its angles), else fewer heads each.

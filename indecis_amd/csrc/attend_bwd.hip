@@ -43,6 +43,7 @@ struct DqShape {
   static constexpr int WAVES = 4, THREADS = 256, ROWS = 128;
   static constexpr int BK = 32;
   typedef Tile<T, DT, BK, THREADS> KV;
+  static_assert(4 * KV::BYTES >= WAVES * 32 * DT * (int)sizeof(T), "the result's rows");
   static constexpr int DOCS = 4 * KV::BYTES, LIVE = DOCS + 2 * 4 * BK, BIAS = LIVE + 8 * kDocWords;
 };
 
@@ -63,7 +64,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : DT == 64 ? 3 : 2) void at
   const int64_t slot = x.slots - 1 - blockIdx.x / a.heads;
   int64_t blk;
   const Seq s = find_block(a, false, ROWS, 1, slot, &blk);
-  if (blk * ROWS >= s.nq) return;
+  if (blk < 0 || blk * ROWS >= s.nq) return;  // below 0: offsets that do not ascend
   const int first = (int)(blk * ROWS);
   const int tok = min(first + wave * 32 + (lane & 31), s.nq - 1);
   const bool mine = first + wave * 32 + (lane & 31) < s.nq;
@@ -246,6 +247,7 @@ struct DkvShape {
   static constexpr int BQ = 32 * SHARE;
   static_assert(KEYS == attend_dkv_keys(sizeof(T), DT), "");
   typedef Tile<T, DT, BQ, THREADS> QO;
+  static_assert(4 * QO::BYTES >= WAVES * 32 * DT * (int)sizeof(T), "the result's rows");
   // Q and dO twice, then lse, delta and the documents of the rows twice
   static constexpr int STAT = 4 * QO::BYTES, DOCS = STAT + 4 * 4 * BQ, LIVE = DOCS + 2 * 4 * BQ,
                        BIAS = LIVE + 8 * kDocWords;
@@ -276,7 +278,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 || DT == 128 ? 1 : 2) void atte
   int64_t blk;
   const Seq s = find_block(a, true, KEYS, 1, blockIdx.x / a.kv_heads, &blk);
   const int64_t slot = blockIdx.x / a.kv_heads;
-  if (blk * KEYS >= s.nk) {
+  if (blk < 0 || blk * KEYS >= s.nk) {
     if (grad_table)
       for (int g = 0; g < x.group; g++)
         for (int i = tid; i < span; i += THREADS) x.dist[(slot * a.heads + kvh * x.group + g) * span + i] = 0.0f;

@@ -45,7 +45,7 @@ void attend_fwd_kernel(AttendArgs x) {
   int64_t blk;
   const Seq s = find_block(a, false, ROWS, pack, x.slots - 1 - blockIdx.x / nh, &blk);
   const int rows = s.nq * pack;
-  if (blk * ROWS >= rows) return;
+  if (blk < 0 || blk * ROWS >= rows) return;  // below 0: offsets that do not ascend
   const int row0 = (int)blk * ROWS, row1 = min(row0 + ROWS, rows);
   const int kvh = pack > 1 ? hb : hb / x.group;
 

@@ -21,21 +21,31 @@ __device__ __forceinline__ void unpack(const F &f, float *x) {
   for (int e = 0; e < 8; e++) x[e] = frag_at(f, e);
 }
 
+// v and the value of another lane of the same 16, by a DPP pattern.
+template <int CTRL>
+__device__ __forceinline__ float add_dpp(float v) {
+  const int o = __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xf, 0xf, true);
+  return v + __builtin_bit_cast(float, o);
+}
+// The sum over LANES lanes, in each of them: neighbours, pairs, then halves
+// and rows of 16 mirrored.
 template <int LANES>
 __device__ __forceinline__ float lanes_sum(float v) {
-#pragma unroll
-  for (int o = 1; o < LANES; o <<= 1) v += __shfl_xor(v, o);
+  v = add_dpp<0xb1>(v);   // quad_perm 1 0 3 2
+  v = add_dpp<0x4e>(v);   // quad_perm 2 3 0 1
+  if constexpr (LANES >= 8) v = add_dpp<0x141>(v);   // row_half_mirror
+  if constexpr (LANES >= 16) v = add_dpp<0x140>(v);  // row_mirror
+  if constexpr (LANES == 32) v += __shfl_xor(v, 16);
   return v;
 }
 
-// The lane's 8 columns of one row: which are there, rotated, and with what.
+// The lane's 8 columns of one row: whether they are there, and their angles.
 template <int LANES>
 struct Lane {
   int c;          // first column
   bool in;        // c < dim
   float co[8], si[8];
   int other;      // lane offset to the rotation's other half; 0: none
-  bool turned[8];
 
   __device__ __forceinline__ Lane(const ixh_norm_rope_args &a, int64_t row, int l) {
     c = 8 * l;
@@ -71,7 +81,7 @@ struct Lane {
       }
     }
   }
-  // y = x rotated; `back` by the opposite angle.
+  // x rotated, by the opposite angle where sign is -1.
   __device__ __forceinline__ void turn(const ixh_norm_rope_args &a, float *x, float sign) const {
     if (a.rot == 0) return;
     float o[8];
@@ -167,7 +177,7 @@ __global__ __launch_bounds__(kThreads) void norm_rope_kernel(NormRopeArgs x) {
 // and heads; the workgroup's groups meet in LDS, the workgroups in
 // norm_rope_gamma_kernel, each in a fixed order.
 template <class T, int LANES, int NORM>
-__global__ __launch_bounds__(kThreads) void norm_rope_backward_kernel(NormRopeArgs x) {
+__global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 3 : 2) void norm_rope_backward_kernel(NormRopeArgs x) {
   typedef typename Kind<T>::frag Frag;
   const ixh_norm_rope_args &a = x.a;
   constexpr int GROUPS = kThreads / LANES;

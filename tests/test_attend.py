@@ -34,6 +34,7 @@ def attend_args(**kw):
     (dict(type=7), "type 7"),
     (dict(B=-1), "-1 sequences"),
     (dict(nq=(1 << 30) + 1), "2\\^30"),
+    (dict(nq=1 << 30, nk=1 << 30, heads=8), "too many rows and heads"),
     (dict(dim=136), "head dimension 136"),
     (dict(dim=12), "head dimension 12"),
     (dict(dim=0), "head dimension 0"),
@@ -125,6 +126,7 @@ def norm_rope_args(**kw):
     (dict(q_heads=-1), "-1 and 2 heads"),
     (dict(dim=264), "head dimension 264"),
     (dict(dim=20), "head dimension 20"),
+    (dict(n=1 << 30), "too many rows for one launch"),
     (dict(norm=3), "norm 3"),
     (dict(eps=-1.0), "eps -1"),
     (dict(eps=float("nan")), "eps nan"),

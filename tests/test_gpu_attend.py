@@ -343,6 +343,28 @@ def test_offsets_out_of_range_read_nothing_out_of_range():
         assert torch.equal(a, b)
 
 
+def test_offsets_that_do_not_ascend_stay_inside():
+    """Whatever the offsets hold, nothing before the first row, past the last,
+    or in a row that no sequence names is written."""
+    rng = np.random.default_rng(27)
+    n = 700
+    q, k, v, do = (rows(rng, torch.bfloat16, n, h, 64) for h in (4, 2, 2, 4))
+    table = rows(rng, torch.bfloat16, 8, 4)
+    kw = dict(table=table, buckets=ints(np.arange(-9, 10) % 8))
+    for offs in ([100, 600, 300, 500, 400], [600, 100, 650, 650, 0], [300, -7, 1 << 30, 200, 600]):
+        room = torch.full((3 * n, 4, 64), 7.0, dtype=torch.bfloat16, device="cuda")
+        grads = [torch.full((3 * n, h, 64), 7.0, dtype=torch.bfloat16, device="cuda") for h in (4, 2, 2)]
+        o = room[n:2 * n]
+        _, lse = attention.attend(q, k, v, ints(offs), out=o, want_lse=True, **kw)
+        lse = torch.where(torch.isnan(lse), 0.0, lse)
+        attention.attend_backward(do, q, k, v, o, lse, ints(offs), dq=grads[0][n:2 * n], dk=grads[1][n:2 * n],
+                                  dv=grads[2][n:2 * n], **kw)
+        torch.cuda.synchronize()
+        for x in (room, *grads):
+            assert (x[:n] == 7).all() and (x[2 * n:] == 7).all()
+            assert (x[n:n + min(max(offs[0], 0), *(max(a, 0) for a in offs))] == 7).all()
+
+
 def test_gradient_against_differences():
     """A float32 loss's central difference along the gradient's own
     direction. h moves the scores by about 1e-2, so the third derivative's
