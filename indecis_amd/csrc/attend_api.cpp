@@ -121,23 +121,37 @@ struct Plan {
   int64_t work;  // bytes of workspace
 };
 
+// Whether the heads that share a key head become rows of one block: it then
+// takes fewer tokens, so that short sequences fill it and masks cut it finer
+// (16/4 heads of 128, 64 sequences, 512 keys, bf16: 1 token 50 -> 22 us, 16
+// tokens 61 -> 33, 32 tokens 68 -> 31). Each head's bias is in LDS.
+int pack_of(const ixh_attend_args &a, int bias_arrays) {
+  const int group = a.heads / a.kv_heads;
+  const bool fits = !a.table || 4LL * group * bias_arrays * attend_bias_len(a.reach) <= 32 << 10;
+  return fits && (int64_t)a.nq * group <= INT32_MAX ? group : 1;
+}
+
 // The forward's kernels. Everything goes by the mean length: the lengths
 // themselves are on the device.
 Plan plan_forward(AttendArgs &x) {
   ixh_attend_args &a = x.a;
   Plan p{};
   x.group = a.heads / a.kv_heads;
-  x.pack = 1;
+  x.pack = pack_of(a, 1);
   const int64_t B = std::max(a.B, 1);
-  if (x.group > 1 && (int64_t)a.nq * x.group <= std::min<int64_t>(32 * B, INT32_MAX) &&
-      (!a.table || 4LL * x.group * attend_bias_len(a.reach) <= 32 << 10))
-    x.pack = x.group;
-  p.few = (int64_t)a.nq * x.pack <= 48 * B;
+  // blocks of one wave where most would have one or two waves' rows (bf16, 12
+  // heads of 64, 256 sequences: 8 tokens 12 against 22 us with four waves, 32
+  // 15 / 25, 64 27 / 29, 96 45 / 37; 16 heads of 128, 64 sequences: 24 tokens
+  // 13 / 16, 48 22 / 20)
+  p.few = (int64_t)a.nq * x.pack <= (a.dim <= 64 ? 64 : 32) * B;
   const int rows = p.few ? kAttendRowsFew : kAttendRowsMany;
   x.slots = attend_slots(a.nq, a.B, rows, x.pack);
   const int64_t groups = x.slots * (x.pack > 1 ? a.kv_heads : a.heads);
   const int64_t steps = a.nk / B / attend_keys(type_size(a.type), p.few);
   x.splits = 1;
+  // few blocks: their keys in parts, until the chip is full (bf16, 12 heads of
+  // 64: 1 query on 512 keys 19 -> 11 us, on 4,096 126 -> 19; 128 queries on
+  // 2,048 48 -> 16, 512 on 4,096 93 -> 29)
   const int64_t want = (p.few ? 8 : 2) * kCus;
   if (groups < want && steps >= 8)
     x.splits = (int)std::min<int64_t>(std::min<int64_t>((want + groups - 1) / std::max<int64_t>(groups, 1), steps / 4),

@@ -255,10 +255,10 @@ void attend_fwd_kernel(AttendArgs x) {
 
 // The parts of the keys joined: a thread has four columns of a query's head.
 template <class T>
-__global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs x) {
+__global__ __launch_bounds__(64) void attend_join_kernel(AttendArgs x) {
   const ixh_attend_args &a = x.a;
   const int quads = a.dim / 4;
-  const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t at = (int64_t)blockIdx.x * 64 + threadIdx.x;
   const int64_t rh = at / quads;
   const int c = (int)(at - rh * quads) * 4;
   const int64_t row = rh / a.heads;
@@ -319,11 +319,11 @@ bool launch_attend_fwd(const AttendArgs &x, bool few, hipStream_t s) {
 
 void launch_attend_join(const AttendArgs &x, hipStream_t s) {
   const int64_t n = (int64_t)x.a.nq * x.a.heads * (x.a.dim / 4);
-  const unsigned grid = (unsigned)((n + 255) / 256);
+  const unsigned grid = (unsigned)((n + 63) / 64);
   switch (x.a.type) {
-    case IXH_TYPE_F32: attend_join_kernel<float><<<grid, 256, 0, s>>>(x); break;
-    case IXH_TYPE_BF16: attend_join_kernel<__bf16><<<grid, 256, 0, s>>>(x); break;
-    default: attend_join_kernel<_Float16><<<grid, 256, 0, s>>>(x); break;
+    case IXH_TYPE_F32: attend_join_kernel<float><<<grid, 64, 0, s>>>(x); break;
+    case IXH_TYPE_BF16: attend_join_kernel<__bf16><<<grid, 64, 0, s>>>(x); break;
+    default: attend_join_kernel<_Float16><<<grid, 64, 0, s>>>(x); break;
   }
 }
 
