@@ -19,7 +19,7 @@ struct AttendArgs {
   ixh_attend_args a;   // as the caller gave them, k_offs and k_docs filled in
   ixh_attend_grads g;  // backward only
   int group;           // heads / kv_heads
-  int pack;            // heads a query row holds in the forward: 1 or group
+  int pack;            // heads of a token that are rows of a block (forward, dQ): 1 or group
   int64_t slots;       // of the launch's row blocks
   int splits;          // parts of the keys (forward)
   float *part_o;       // [splits][nq][heads][dim], unnormalised

@@ -125,9 +125,9 @@ struct Plan {
 // takes fewer tokens, so that short sequences fill it and masks cut it finer
 // (16/4 heads of 128, 64 sequences, 512 keys, bf16: 1 token 50 -> 22 us, 16
 // tokens 61 -> 33, 32 tokens 68 -> 31). Each head's bias is in LDS.
-int pack_of(const ixh_attend_args &a, int bias_arrays) {
+int pack_of(const ixh_attend_args &a) {
   const int group = a.heads / a.kv_heads;
-  const bool fits = !a.table || 4LL * group * bias_arrays * attend_bias_len(a.reach) <= 32 << 10;
+  const bool fits = !a.table || 4LL * group * attend_bias_len(a.reach) <= 32 << 10;
   return fits && (int64_t)a.nq * group <= INT32_MAX ? group : 1;
 }
 
@@ -137,7 +137,7 @@ Plan plan_forward(AttendArgs &x) {
   ixh_attend_args &a = x.a;
   Plan p{};
   x.group = a.heads / a.kv_heads;
-  x.pack = pack_of(a, 1);
+  x.pack = pack_of(a);
   const int64_t B = std::max(a.B, 1);
   // blocks of one wave where most would have one or two waves' rows (bf16, 12
   // heads of 64, 256 sequences: 8 tokens 12 against 22 us with four waves, 32
@@ -165,8 +165,8 @@ Plan plan_forward(AttendArgs &x) {
 int64_t plan_backward(AttendArgs &x, int64_t *key_slots) {
   const ixh_attend_args &a = x.a;
   x.group = a.heads / a.kv_heads;
-  x.pack = 1;
-  x.slots = attend_slots(a.nq, a.B, 128, 1);
+  x.pack = pack_of(a);
+  x.slots = attend_slots(a.nq, a.B, 128, x.pack);
   *key_slots = attend_slots(a.nk, a.B, attend_dkv_keys(type_size(a.type), a.dim), 1);
   int64_t bytes = up(4LL * a.heads * a.nq);
   x.dist_parts = 0;

@@ -60,26 +60,29 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : DT == 64 ? 3 : 2) void at
   int *const kdocs = (int *)(smem + Sh::DOCS);
   uint64_t *const live = (uint64_t *)(smem + Sh::LIVE);
   float *const bias = (float *)(smem + Sh::BIAS);
-  const int head = blockIdx.x % a.heads, kvh = head / x.group;
-  const int64_t slot = x.slots - 1 - blockIdx.x / a.heads;
+  const int pack = x.pack, nh = pack > 1 ? a.kv_heads : a.heads;
+  const int hb = blockIdx.x % nh, kvh = pack > 1 ? hb : hb / x.group;
   int64_t blk;
-  const Seq s = find_block(a, false, ROWS, 1, slot, &blk);
-  if (blk < 0 || blk * ROWS >= s.nq) return;  // below 0: offsets that do not ascend
-  const int first = (int)(blk * ROWS);
-  const int tok = min(first + wave * 32 + (lane & 31), s.nq - 1);
-  const bool mine = first + wave * 32 + (lane & 31) < s.nq;
+  const Seq s = find_block(a, false, ROWS, pack, x.slots - 1 - blockIdx.x / nh, &blk);
+  const int rows = s.nq * pack;
+  if (blk < 0 || blk * ROWS >= rows) return;  // below 0: offsets that do not ascend
+  const int row0 = (int)blk * ROWS, row1 = min(row0 + ROWS, rows);
+  auto token = [&](int r) { return pack > 1 ? r / pack : r; };
+  const int r = min(row0 + wave * 32 + (lane & 31), rows - 1), tok = token(r), sub = r - tok * pack;
+  const int head = pack > 1 ? hb * pack + sub : hb;
+  const bool mine = row0 + wave * 32 + (lane & 31) < rows;
   const int p = tok + s.shift;
   int lo, hi;
   key_bounds(a, s, p, &lo, &hi);
   const int p_lo = __builtin_amdgcn_readlane(p, 0), p_hi = __builtin_amdgcn_readlane(p, 31);
   const int lo_min = __builtin_amdgcn_readlane(lo, 0), lo_max = __builtin_amdgcn_readlane(lo, 31);
   const int hi_min = __builtin_amdgcn_readlane(hi, 0);
-  const int hi_max = first + wave * 32 < s.nq ? __builtin_amdgcn_readlane(hi, 31) : -1;
+  const int hi_max = row0 + wave * 32 < rows ? __builtin_amdgcn_readlane(hi, 31) : -1;
   int t_begin, t_end;
   {
     int l, u, unused;
-    key_bounds(a, s, first + s.shift, &l, &unused);
-    key_bounds(a, s, min(first + ROWS, s.nq) - 1 + s.shift, &unused, &u);
+    key_bounds(a, s, token(row0) + s.shift, &l, &unused);
+    key_bounds(a, s, token(row1 - 1) + s.shift, &unused, &u);
     t_begin = l / BK;
     t_end = u >= l ? u / BK + 1 : t_begin;
   }
@@ -112,14 +115,16 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : DT == 64 ? 3 : 2) void at
   const T *const vb = (const T *)a.v.p + s.k0 * a.v.row + kvh * a.v.head;
   const Score sc(a, FEAT & kCap);
   const float unit = bias_unit(a, FEAT & kCap);
-  const Bias by{(FEAT & kBias) && a.table ? bias : nullptr,
+  const Bias by{(FEAT & kBias) && a.table ? bias + sub * attend_bias_len(a.reach) : nullptr,
                 (FEAT & kBias) && a.slopes ? -a.slopes[head] * unit : 0.0f, a.reach};
   if constexpr (FEAT & kBias) {
-    if (a.table) load_bias<T>(a, head, unit, bias, tid, THREADS);
+    if (a.table)
+      for (int i = 0; i < pack; i++)
+        load_bias<T>(a, pack > 1 ? hb * pack + i : hb, unit, bias + i * attend_bias_len(a.reach), tid, THREADS);
   }
   if (a.q_docs)
-    doc_steps<BK, Sh::WAVES>(a.q_docs + s.q0, first, min(first + ROWS, s.nq) - 1, a.k_docs + s.k0, s.nk, t_begin, t_end,
-                             live, wave, lane);
+    doc_steps<BK, Sh::WAVES>(a.q_docs + s.q0, token(row0), token(row1 - 1), a.k_docs + s.k0, s.nk, t_begin, t_end, live,
+                             wave, lane);
   if (a.q_docs || (FEAT & kBias)) __syncthreads();
   auto next = [&](int t) { return a.q_docs ? next_live(live, t, t_begin, t_end) : t; };
   float row_sum = 0.0f;  // of dZ
@@ -227,8 +232,9 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : DT == 64 ? 3 : 2) void at
   row_sum = half_sum(row_sum);
   if (mine && h == 0) x.delta[(int64_t)head * a.nq + row] = delta + row_sum;
   store_rows<T, DT>(acc, a.scale, smem + wave * (32 * DT * (int)sizeof(T)), a.dim, lane, [&](int i) {
-    const int r = first + wave * 32 + i;
-    return r < s.nq ? (T *)x.g.dq.p + (int64_t)(s.q0 + r) * x.g.dq.row + head * x.g.dq.head : (T *)nullptr;
+    const int r = row0 + wave * 32 + i, tok = token(r);
+    if (r >= rows) return (T *)nullptr;
+    return (T *)x.g.dq.p + (int64_t)(s.q0 + tok) * x.g.dq.row + (pack > 1 ? hb * pack + r - tok * pack : hb) * x.g.dq.head;
   });
 }
 
@@ -639,10 +645,10 @@ template <class T, int DT, int FEAT>
 bool run_dq(const AttendArgs &x, hipStream_t s) {
   typedef DqShape<T, DT> Sh;
   const int len = (FEAT & kBias) && x.a.table ? attend_bias_len(x.a.reach) : 0;
-  const int shm = Sh::BIAS + 4 * len;
+  const int shm = Sh::BIAS + 4 * x.pack * len;
   static PerDevice lds;
   if (!lds_granted(lds, (const void *)attend_dq_kernel<T, DT, FEAT>, 160 << 10)) return false;
-  attend_dq_kernel<T, DT, FEAT><<<dim3((unsigned)(x.slots * x.a.heads)), Sh::THREADS, shm, s>>>(x);
+  attend_dq_kernel<T, DT, FEAT><<<dim3((unsigned)(x.slots * (x.pack > 1 ? x.a.kv_heads : x.a.heads))), Sh::THREADS, shm, s>>>(x);
   return true;
 }
 template <class T, int DT, int FEAT>
