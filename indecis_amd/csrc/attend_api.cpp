@@ -381,7 +381,7 @@ void plan_norm_rope(NormRopeArgs &x, bool backward) {
   const int heads = std::max(x.a.q_heads + x.a.k_heads, 1);
   const int64_t groups = 256 / row_lanes(x.a.dim);
   const int64_t blocks = std::max<int64_t>((x.a.n + groups - 1) / groups, 1);
-  const int64_t want = 8 * kCus;  // workgroups
+  const int64_t want = 4 * kCus;  // workgroups
   x.heads_step = (int)std::min<int64_t>(heads, std::max<int64_t>(1, blocks * heads / want));
   x.blocks = (int)(backward ? std::min<int64_t>(blocks, kNormRopeBlocks) : blocks);
 }
