@@ -19,6 +19,7 @@ struct AttendArgs {
   ixh_attend_args a;   // as the caller gave them, k_offs and k_docs filled in
   ixh_attend_grads g;  // backward only
   int group;           // heads / kv_heads
+  int share;           // waves that have the same 32 keys in the dK, dV kernel: 1 or 2
   int pack;            // heads of a token that are rows of a block (forward, dQ): 1 or group
   int64_t slots;       // of the launch's row blocks
   int splits;          // parts of the keys (forward)
@@ -38,9 +39,6 @@ constexpr int attend_keys(int size, bool few) { return size == 4 || few ? 32 : 6
 // row of the table's copy in LDS needs no clamped index.
 constexpr int kBiasPad = 96;
 constexpr int attend_bias_len(int reach) { return 2 * (reach + kBiasPad) + 1; }
-
-// Keys a workgroup of the dK, dV kernel.
-constexpr int attend_dkv_keys(int type_size, int dim) { return (type_size == 2) == (dim > 64) ? 64 : 128; }
 
 bool launch_attend_fwd(const AttendArgs &x, bool few, hipStream_t s);
 void launch_attend_join(const AttendArgs &x, hipStream_t s);

@@ -161,13 +161,31 @@ Plan plan_forward(AttendArgs &x) {
   return p;
 }
 
+// Waves that share 32 keys in the dK, dV kernel. Two, for more blocks, where
+// one workgroup's sums take a CU (over 64 columns of 16 bits: 8 sequences of
+// 2,048, 16/4 heads of 128, documents, forward and backward 1,015 -> 817 us; 8
+// heads, 64 sequences of 512, 652 -> 690; float32 to 64 columns: 24 sequences
+// of 33-300, 6 heads, 185 -> 172, 8 of 2,048, 8 heads, 2,950 -> 3,070).
+// float32 past 64 columns has no LDS for it. 16 bits to 64 columns leave two
+// workgroups a CU: two waves share where there are no more than that, or,
+// with a key head a query head and so shorter blocks, half as many (bf16,
+// heads of 64: 8 of 2,048, 8/2 heads, 597 -> 469; 64 of 512, 8/2, 311 -> 290,
+// 64 of 2,048 3,390 -> 3,545; 2 of 2,048, 8/8, 220 -> 192, 4 of 1,024, 12/12,
+// 132 -> 135).
+int share_of(const ixh_attend_args &a) {
+  if (type_size(a.type) == 4) return a.dim > 64 ? 1 : 2;
+  if (a.dim > 64) return 2;
+  return (int64_t)a.nk * a.kv_heads <= 128LL * kCus * (a.heads > a.kv_heads ? 2 : 1) ? 2 : 1;
+}
+
 // The dQ kernel's slots in x; the dK, dV kernel's in *key_slots.
 int64_t plan_backward(AttendArgs &x, int64_t *key_slots) {
   const ixh_attend_args &a = x.a;
   x.group = a.heads / a.kv_heads;
   x.pack = pack_of(a);
   x.slots = attend_slots(a.nq, a.B, 128, x.pack);
-  *key_slots = attend_slots(a.nk, a.B, attend_dkv_keys(type_size(a.type), a.dim), 1);
+  x.share = share_of(a);
+  *key_slots = attend_slots(a.nk, a.B, 128 / x.share, 1);
   int64_t bytes = up(4LL * a.heads * a.nq);
   x.dist_parts = 0;
   if (a.table) {

@@ -240,18 +240,14 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : DT == 64 ? 3 : 2) void at
 
 // ---- dK, dV -----------------------------------------------------------------
 
-// Four waves have 128 keys, 32 each, and 32 queries a step. Where the sums of
-// a wave take the registers of a whole SIMD (head dimensions over 64, or
-// float32), few blocks run at once, and a block of keys that many queries see
-// holds up the launch: there two waves share 32 keys, each with every other
-// 32 queries of a step of 64, and add their sums up at the end (8 sequences
-// of 2,048, 16/4 heads of 128, documents of up to 1,500: 441 -> 260 us).
-template <class T, int DT>
+// Four waves have 128 keys, 32 each, and 32 queries a step. A block of keys
+// that many queries see holds up a launch of few blocks: there two waves
+// share 32 keys (SHARE 2), each with every other 32 queries of a step of 64,
+// and add their sums up at the end. attend_api.cpp says when.
+template <class T, int DT, int SHARE>
 struct DkvShape {
-  static constexpr int SHARE = (sizeof(T) == 2) == (DT == 128) ? 2 : 1;
   static constexpr int WAVES = 4, THREADS = 256, KEYS = 128 / SHARE;
   static constexpr int BQ = 32 * SHARE;
-  static_assert(KEYS == attend_dkv_keys(sizeof(T), DT), "");
   typedef Tile<T, DT, BQ, THREADS> QO;
   static_assert(4 * QO::BYTES >= WAVES * 32 * DT * (int)sizeof(T), "the result's rows");
   // Q and dO twice, then lse, delta and the documents of the rows twice
@@ -259,9 +255,9 @@ struct DkvShape {
                        BIAS = LIVE + 8 * kDocWords;
 };
 
-template <class T, int DT, int FEAT>
+template <class T, int DT, int FEAT, int SHARE>
 __global__ __launch_bounds__(256, sizeof(T) == 4 || DT == 128 ? 1 : 2) void attend_dkv_kernel(AttendArgs x) {
-  typedef DkvShape<T, DT> Sh;
+  typedef DkvShape<T, DT, SHARE> Sh;
   typedef typename Sh::QO QO;
   typedef typename Kind<T>::frag Frag;
   constexpr int THREADS = Sh::THREADS, KEYS = Sh::KEYS, BQ = Sh::BQ, KS = DT / 16, ND = DT / 32;
@@ -269,7 +265,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 || DT == 128 ? 1 : 2) void atte
   const ixh_attend_args &a = x.a;
   const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int kw = wave / Sh::SHARE, qw = wave % Sh::SHARE;  // the wave's keys, its queries of a step
+  const int kw = wave / SHARE, qw = wave % SHARE;  // the wave's keys, its queries of a step
   float *const stat = (float *)(smem + Sh::STAT);
   int *const qdocs = (int *)(smem + Sh::DOCS);
   uint64_t *const live = (uint64_t *)(smem + Sh::LIVE);
@@ -551,7 +547,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 || DT == 128 ? 1 : 2) void atte
     }
     g = then_g, t = then;
   }
-  if constexpr (Sh::SHARE == 2) {
+  if constexpr (SHARE == 2) {
     // the second wave's sums, through LDS to the first: dK's, then dV's
     static_assert(4 * QO::BYTES >= 2 * 64 * 16 * ND * 4, "");
     f4 *const sums = (f4 *)smem + kw * 64 * 4 * ND + lane;
@@ -651,15 +647,24 @@ bool run_dq(const AttendArgs &x, hipStream_t s) {
   attend_dq_kernel<T, DT, FEAT><<<dim3((unsigned)(x.slots * (x.pack > 1 ? x.a.kv_heads : x.a.heads))), Sh::THREADS, shm, s>>>(x);
   return true;
 }
-template <class T, int DT, int FEAT>
-bool run_dkv(const AttendArgs &x, hipStream_t s) {
-  typedef DkvShape<T, DT> Sh;
+template <class T, int DT, int FEAT, int SHARE>
+bool run_dkv_shared(const AttendArgs &x, hipStream_t s) {
+  typedef DkvShape<T, DT, SHARE> Sh;
   const int len = (FEAT & kBias) && x.a.table ? attend_bias_len(x.a.reach) : 0;
   const int shm = Sh::BIAS + 4 * len * (2 + Sh::WAVES);
   static PerDevice lds;
-  if (!lds_granted(lds, (const void *)attend_dkv_kernel<T, DT, FEAT>, 160 << 10)) return false;
-  attend_dkv_kernel<T, DT, FEAT><<<dim3((unsigned)(x.slots * x.a.kv_heads)), Sh::THREADS, shm, s>>>(x);
+  if (!lds_granted(lds, (const void *)attend_dkv_kernel<T, DT, FEAT, SHARE>, 160 << 10)) return false;
+  attend_dkv_kernel<T, DT, FEAT, SHARE><<<dim3((unsigned)(x.slots * x.a.kv_heads)), Sh::THREADS, shm, s>>>(x);
   return true;
+}
+template <class T, int DT, int FEAT>
+bool run_dkv(const AttendArgs &x, hipStream_t s) {
+  if constexpr (sizeof(T) == 4 && DT == 128)
+    return run_dkv_shared<T, DT, FEAT, 1>(x, s);
+  else if constexpr (sizeof(T) == 2 && DT == 64)
+    return x.share == 1 ? run_dkv_shared<T, DT, FEAT, 1>(x, s) : run_dkv_shared<T, DT, FEAT, 2>(x, s);
+  else
+    return run_dkv_shared<T, DT, FEAT, 2>(x, s);
 }
 
 template <class T, int DT>

@@ -16,6 +16,12 @@ sums round), w = 2^-24 half a step of float32.
  - dZ = P (dP - delta): delta is taken of the rounded o, so it is off by
    |dO| times o's bound; dP is a sum of dim products.
  - dQ, dK, dV: dZ (P) rounded to the type, the 32-bit sum, one last rounding.
+ - below 2^-14 float16's values are 2^-24 apart, so that each rounding to it
+   may be off by half of that, 2^-25, whatever the value (a key whose only
+   query sees nothing else has dZ = 0 but for delta's own rounding, and a dK
+   of some 1e-8): 2^-25 for a result, and for each P and dZ that it sums,
+   times the other factor. bfloat16 and float32 have normal values down to
+   2^-126: their share is inside the 1e-30.
 Every second-order term is covered by a factor of 1.05."""
 import math
 
@@ -55,6 +61,7 @@ def attend(q, k, v, q_offs, k_offs, *, u, scale=None, cap=0.0, slopes=None, tabl
     nq, heads, dim = q.shape
     group = heads // k.shape[1]
     scale = dim ** -0.5 if scale is None else scale
+    tiny = 2.0 ** -25 if u == 2.0 ** -11 else 1e-30  # a rounding below the type's normal values
     tanh_err = 4 * W if u == 0 else 2.0 ** -20
     out = {n: [np.full(s, np.nan), np.zeros(s)] for n, s in
            (("o", q.shape), ("lse", (heads, nq)), ("dq", q.shape), ("dk", k.shape), ("dv", v.shape))}
@@ -92,7 +99,7 @@ def attend(q, k, v, q_offs, k_offs, *, u, scale=None, cap=0.0, slopes=None, tabl
             worst = np.where(see, ez, 0).max(1, initial=0)[:, None]
             ep = 2 * worst + (m + 16) * W  # relative, of p
             o, ov = p @ vh, p @ np.abs(vh)
-            eo = 1.05 * (u * np.abs(o) + (u + ep + W * m) * ov + W * np.abs(o)) + 1e-30
+            eo = 1.05 * (u * np.abs(o) + (u + ep + W * m) * ov + W * np.abs(o) + tiny * (see @ np.abs(vh))) + tiny
             out["o"][0][q0:q1, h], out["o"][1][q0:q1, h] = o, eo
             with np.errstate(divide="ignore"):
                 lse = np.where(seen, top[:, 0] + np.log(total[:, 0]), -np.inf)
@@ -117,11 +124,11 @@ def attend(q, k, v, q_offs, k_offs, *, u, scale=None, cap=0.0, slopes=None, tabl
             ds = dz * slope
             # 1 - tanh^2 from the reciprocal, absolutely as near as tanh
             eds = edz * np.abs(slope) + (0 if cap == 0 else 4 * (tanh_err + 4 * W) + 2 * es / cap) * np.abs(dz)
-            size = (u + (m + n + 8) * W) * np.abs(ds) + eds
+            size = (u + (m + n + 8) * W) * np.abs(ds) + eds + tiny * see
             for name, val, err, sl, hh in (
                     ("dq", scale * (ds @ kh), scale * (size @ np.abs(kh)), slice(q0, q1), h),
                     ("dk", scale * (ds.T @ qh), scale * (size.T @ np.abs(qh)), slice(k0, k1), g),
-                    ("dv", p.T @ do, ((u + ep + (n + 8) * W) * p).T @ np.abs(do), slice(k0, k1), g)):
+                    ("dv", p.T @ do, ((u + ep + (n + 8) * W) * p + tiny * see).T @ np.abs(do), slice(k0, k1), g)):
                 if name == "dq" or h % group == 0:
                     out[name][0][sl, hh] = 0
                 out[name][0][sl, hh] += val
@@ -129,10 +136,10 @@ def attend(q, k, v, q_offs, k_offs, *, u, scale=None, cap=0.0, slopes=None, tabl
     res = {"o": out["o"], "lse": out["lse"]}
     if d_out is not None:
         for name in ("dq", "dk", "dv"):
-            out[name][1] += (u + W) * np.nan_to_num(np.abs(out[name][0])) + 1e-30
+            out[name][1] += (u + W) * np.nan_to_num(np.abs(out[name][0])) + tiny
             res[name] = out[name]
         if dtable is not None:
-            dtable[1] = 1.05 * dtable[1] + (u + W) * np.abs(dtable[0]) + 1e-30
+            dtable[1] = 1.05 * dtable[1] + (u + W) * np.abs(dtable[0]) + tiny
             res["dtable"] = dtable
     return res
 

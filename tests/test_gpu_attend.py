@@ -178,6 +178,28 @@ def test_heads(heads, kv_heads):
           slopes=ref.alibi(heads))
 
 
+@pytest.mark.parametrize("t", ["bf16", "f16"])
+@pytest.mark.parametrize("name", ["plain", "cap", "table", "all"])
+@pytest.mark.parametrize("heads,copies", [(40, 1), (80, 2)])
+def test_keys_past_two_workgroups_a_cu(t, name, heads, copies):
+    """Gradients over more keys and key heads than the blocks of 64 keys are
+    taken for, a key head each head and shared."""
+    lens = [200, 129, 1, 90, 0, 64, 300, 33, 70] * copies
+    kv_heads = 40
+    assert sum(lens) * kv_heads > 128 * 256 * (heads // kv_heads)
+    rng = np.random.default_rng(22)
+    kw = {}
+    if name in ("cap", "all"):
+        kw["cap"] = 4.0
+    if name in ("table", "all"):
+        kw.update(table=rng.standard_normal((8, heads)), buckets=np.arange(-20, 21) % 8)
+    if name == "all":
+        docs = np.sort(rng.integers(0, 9, sum(lens)))
+        docs[-12:] = -1
+        kw.update(slopes=ref.alibi(heads), causal=True, window=90, docs=docs)
+    check(rng, t, lens, heads=heads, kv_heads=kv_heads, dim=32, **kw)
+
+
 @pytest.mark.parametrize("t", TYPES)
 @pytest.mark.parametrize("heads,kv_heads,dim", [(4, 4, 64), (8, 2, 128), (8, 1, 72), (40, 1, 64)])
 def test_one_token(t, heads, kv_heads, dim):
