@@ -38,6 +38,12 @@ __device__ __forceinline__ float shape_scores(v16f &z, float *slope_of, const Sc
 
 // ---- dQ ---------------------------------------------------------------------
 
+// As the forward: a lane has a query (row), K and V come through LDS, 32 keys
+// a step. S^T, dP^T and dQ (twice, for dS in two pieces) are its products.
+// Bound by the issue of vector and matrix instructions (8 sequences of 2,048,
+// 16/4 heads of 128, bf16, documents, causal, cap: 245-260 us; 48 sequences of
+// 64-512, 12 heads of 64, learned bias: 75 us).
+
 template <class T, int DT>
 struct DqShape {
   static constexpr int WAVES = 4, THREADS = 256, ROWS = 128;
@@ -244,6 +250,14 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : DT == 64 ? 3 : 2) void at
 // that many queries see holds up a launch of few blocks: there two waves
 // share 32 keys (SHARE 2), each with every other 32 queries of a step of 64,
 // and add their sums up at the end. attend_api.cpp says when.
+// A lane has a key, whose dK and dV stay in registers; K and V are fragments
+// in registers, Q and dO come through LDS for both uses, by rows for S and dP,
+// transposed for dK and dV. At heads over 64 the sums take a SIMD's registers,
+// so that one wave's products, vector work and LDS reads follow one another
+// (about 2.7 us a step of 64 queries): that, not a rate, is what bounds it (8
+// sequences of 2,048, 16/4 heads of 128, bf16, documents, causal, cap: 410-430
+// us; 48 sequences of 64-512, 12 heads of 64, learned bias with its gradient:
+// 118 us; 24 of 33-300, 6 heads of 48, float32: 67).
 template <class T, int DT, int SHARE>
 struct DkvShape {
   static constexpr int WAVES = 4, THREADS = 256, KEYS = 128 / SHARE;
@@ -587,7 +601,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 || DT == 128 ? 1 : 2) void atte
 // ---- the table's gradient ----------------------------------------------------
 
 // Sums of dZ by distance over the workgroups of attend_dkv_kernel: a part of
-// them each block, four strands a distance.
+// them each block, four strands a distance. Bound by latency (12 heads, reach
+// 128, 160 workgroups a head: 4.8 us).
 __global__ __launch_bounds__(256) void attend_dist_kernel(AttendArgs x) {
   __shared__ float strand[4][64];
   const int span = 2 * x.a.reach + 1, head = blockIdx.y, part = blockIdx.z;
@@ -605,7 +620,8 @@ __global__ __launch_bounds__(256) void attend_dist_kernel(AttendArgs x) {
 }
 
 // The distances of each bucket: a block a head, 256 / n_buckets strands a
-// bucket (at least one), each of its distances in ascending order.
+// bucket (at least one), each of its distances in ascending order. Bound by
+// the latency of its dependent steps (12 heads, reach 128, 32 buckets: 10 us).
 template <class T>
 __global__ __launch_bounds__(256) void attend_dtable_kernel(AttendArgs x) {
   extern __shared__ __attribute__((aligned(16))) char smem[];

@@ -263,7 +263,8 @@ struct Tile {
 // A wave's 32 result rows (lane l has row l % 32, columns as the registers
 // hold them) times f, through 32 rows of its own in LDS to whole rows in
 // memory: eight bytes a lane of a row each would cost the address unit a
-// cycle a lane, 45 us of a launch of 9,864 blocks. row_at(i): the address of
+// cycle a lane (256 sequences of 64-512, 12 heads of 64, window of 64: 162 ->
+// 156 us). row_at(i): the address of
 // row i, or nullptr. Every wave calls it, the block's tiles no longer needed.
 template <class T, int DT, class RowAt>
 __device__ __forceinline__ void store_rows(const v16f *acc, float f, char *lds, int dim, int lane, RowAt row_at) {

@@ -7,6 +7,20 @@
 // The scores are taken transposed (keys x queries, attend_device.h): a lane
 // has one query, so maximum, sum and rescaling are its own, and the
 // probabilities go into the second product from the registers they are in.
+//
+// What bounds it, by the shape (bf16, heads of 64 unless said otherwise; the
+// card's copy 4.9 TB/s, a large product 1,060 TFLOP/s):
+//  - long sequences: the issue of matrix and vector instructions together (4
+//    sequences of 8,192, 12 heads, causal with prefix: 570 us, 742 TFLOP/s);
+//  - many short blocks: a block's start, its few steps in series, and the
+//    vector work of cap and masks (256 sequences of 64-512, 12 heads, cap and
+//    window of 64: 146 us, 3.1 TB/s; learned bias, no window: 205 us, 369
+//    TFLOP/s);
+//  - one token over long keys: the reading of K and V (32 sequences of
+//    512-8,192, 16/4 heads of 128, float16: 67 us and the join's 9, 2.8 TB/s
+//    of the whole call);
+//  - one short sequence: its block's steps in series (15 tokens, 4 heads,
+//    float32: 9 us).
 #include "attend_device.h"
 #include "ixh_internal.h"
 
@@ -253,7 +267,9 @@ void attend_fwd_kernel(AttendArgs x) {
   });
 }
 
-// The parts of the keys joined: a thread has four columns of a query's head.
+// The parts of the keys joined: a thread has four columns of a query's head,
+// which it adds up over the parts in their order. Bound by latency: the parts'
+// maxima, then their rows (32 x 16 heads of 128, 8.9 us).
 template <class T>
 __global__ __launch_bounds__(64) void attend_join_kernel(AttendArgs x) {
   const ixh_attend_args &a = x.a;

@@ -6,7 +6,9 @@
 // are shuffles inside those lanes, and a rotation by halves takes its other
 // value from the lane rot / 16 away. A lane keeps its angles and gammas in
 // registers over the heads of a row. All arithmetic is in 32 bits; a result
-// is rounded once.
+// is rounded once. Measured: 72,500 rows of 12+12 heads of 64, bf16, 95 us,
+// 4.7 TB/s (the card's copy 4.9); 16,384 rows of 16+4 heads of 128, float16,
+// forward and gradients 101 us, 4.2 TB/s; 15 rows 3.8 us, the launch.
 #include "attend_device.h"
 #include "ixh_internal.h"
 
@@ -175,7 +177,8 @@ __global__ __launch_bounds__(kThreads) void norm_rope_kernel(NormRopeArgs x) {
 
 // The gradients. A lane adds up its columns' gamma gradients over its rows
 // and heads; the workgroup's groups meet in LDS, the workgroups in
-// norm_rope_gamma_kernel, each in a fixed order.
+// norm_rope_gamma_kernel, each in a fixed order. Three waves a SIMD, for
+// loads in flight (16,384 rows of 16+4 heads of 128, float16: 55 us).
 template <class T, int LANES, int NORM>
 __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 3 : 2) void norm_rope_backward_kernel(NormRopeArgs x) {
   typedef typename Kind<T>::frag Frag;
@@ -259,6 +262,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 3 : 2) void norm_rope_ba
 }
 
 // A block has 4 columns of one gamma, a thread every 256th part of them.
+// Bound by latency (512 workgroups' parts of 128 columns: 6 us).
 __global__ __launch_bounds__(256) void norm_rope_gamma_kernel(NormRopeArgs x, int parts) {
   __shared__ f4 strand[4];
   const ixh_norm_rope_args &a = x.a;
