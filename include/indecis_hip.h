@@ -462,7 +462,8 @@ int ixh_attend(int device, const ixh_attend_args *a, void *stream);
  * them: dq, dk (over the heads that share it), dv, and the table's. In
  * float16 a score's gradient, P (dP - sum dO o), has to stay in the type's
  * range, as a scaled loss keeps it. The workspace of a table's gradient grows
- * with keys / 64 * heads * (2 reach + 1) * 4 bytes. */
+ * with keys / 64 * heads * (2 reach + 1) * 4 bytes; few long sequences, which
+ * are computed in parts, take up to some 100 MiB. */
 int ixh_attend_backward(int device, const ixh_attend_args *a, const ixh_attend_grads *g, void *stream);
 
 /* The buckets of a learned distance bias, map [2 max_distance + 1] for

@@ -22,11 +22,13 @@ struct AttendArgs {
   int share;           // waves that have the same 32 keys in the dK, dV kernel: 1 or 2
   int pack;            // heads of a token that are rows of a block (forward, dQ): 1 or group
   int64_t slots;       // of the launch's row blocks
-  int splits;          // parts of the keys (forward)
-  float *part_o;       // [splits][nq][heads][dim], unnormalised
+  int splits;          // parts of the keys (forward, dQ), of the queries (dK, dV)
+  float *part_o;       // [splits][nq][heads][dim], unnormalised; the backward's
+                       // too, and [splits][2][nk][kv_heads][dim] for dK and dV
   float *part_ml;      // [splits][nq][heads][2]: maximum (base 2) and sum
   float *delta;        // [heads][nq]: sum of dO * o (backward)
-  float *dist;         // [slots][heads][2 reach + 1]: sums of dZ by distance (backward)
+  float *part_delta;   // [splits][heads][nq]
+  float *dist;         // [slots * splits][heads][2 reach + 1]: sums of dZ by distance (backward)
   float *dist_sum;     // [parts][heads][2 reach + 1]
   int dist_parts;
 };
@@ -44,6 +46,8 @@ bool launch_attend_fwd(const AttendArgs &x, bool few, hipStream_t s);
 void launch_attend_join(const AttendArgs &x, hipStream_t s);
 bool launch_attend_dq(const AttendArgs &x, hipStream_t s);
 bool launch_attend_dkv(const AttendArgs &x, hipStream_t s);
+// The parts of dQ and delta, or of dK and dV, added up.
+void launch_attend_sum(const AttendArgs &x, bool keys, hipStream_t s);
 void launch_attend_dtable(const AttendArgs &x, hipStream_t s);
 
 struct NormRopeArgs {

@@ -178,21 +178,64 @@ int share_of(const ixh_attend_args &a) {
   return (int64_t)a.nk * a.kv_heads <= 128LL * kCus * (a.heads > a.kv_heads ? 2 : 1) ? 2 : 1;
 }
 
-// The dQ kernel's slots in x; the dK, dV kernel's in *key_slots.
-int64_t plan_backward(AttendArgs &x, int64_t *key_slots) {
+// The backward's parts for `groups` workgroups of `steps` steps, each `heads`
+// heads long: of at least four steps in float32 and eight in 16 bits until
+// there are `want` workgroups a CU, and of at least 16 until there are twice
+// as many; not where they save a workgroup less than 3 (12) steps, as the
+// parts' sums go through memory and a launch of their own. Forward and
+// backward, heads of 64: 1 sequence of 2,048, 2 heads, float32, 460 -> 135
+// us; 1 of 2,048, 4 heads, bf16, 130 -> 86; 1 of 8,192, 2 heads, float16, 455 ->
+// 246; 2 of 4,096, 12 heads, float16, 448 -> 462; 8 of 512, 6 heads, bf16, in
+// parts of eight steps 67, without 63.
+int splits_of(const ixh_attend_args &a, int64_t groups, int64_t steps, int heads, int64_t want) {
+  const bool wide = type_size(a.type) == 4;
+  auto parts = [&](int64_t workgroups, int least) -> int64_t {
+    if (groups >= workgroups) return 1;
+    least = std::max(least / heads, 2);
+    const int64_t n = std::min<int64_t>({(workgroups + groups - 1) / std::max<int64_t>(groups, 1), steps / least, kMaxSplits});
+    return n > 1 && steps * heads * (n - 1) >= n * (wide ? 3 : 12) ? n : 1;
+  };
+  return (int)std::max(parts(want * kCus, wide ? 4 : 8), parts(2 * want * kCus, 16));
+}
+
+// The backward's launches: x the dQ kernel's, y the dK, dV kernel's. Returns
+// the bytes of workspace, the pointers into it set from x.a.workspace.
+int64_t plan_backward(AttendArgs &x, AttendArgs &y) {
   const ixh_attend_args &a = x.a;
+  const int64_t B = std::max(a.B, 1);
   x.group = a.heads / a.kv_heads;
   x.pack = pack_of(a);
-  x.slots = attend_slots(a.nq, a.B, 128, x.pack);
   x.share = share_of(a);
-  *key_slots = attend_slots(a.nk, a.B, 128 / x.share, 1);
-  int64_t bytes = up(4LL * a.heads * a.nq);
+  x.slots = attend_slots(a.nq, a.B, 128, x.pack);
   x.dist_parts = 0;
+  y = x;
+  y.slots = attend_slots(a.nk, a.B, 128 / x.share, 1);
+  x.splits = splits_of(a, x.slots * (x.pack > 1 ? a.kv_heads : a.heads), a.nk / B / 32, 1, type_size(a.type) == 4 ? 1 : 2);
+  y.splits = splits_of(a, y.slots * a.kv_heads, a.nq / B / (32 * x.share), x.group, 1);
+
+  char *const w = (char *)a.workspace;
+  int64_t bytes = 0;
+  auto take = [&](int64_t n) {
+    const int64_t at = bytes;
+    bytes += up(4 * n);
+    return w ? (float *)(w + at) : nullptr;
+  };
+  x.delta = y.delta = take((int64_t)a.heads * a.nq);
   if (a.table) {
     const int64_t span = 2LL * a.reach + 1;
-    x.dist_parts = kMaxDistParts;
-    bytes += up(4 * *key_slots * a.heads * span) + up(4 * x.dist_parts * a.heads * span);
+    y.dist_parts = kMaxDistParts;
+    y.dist = take(y.slots * y.splits * a.heads * span);
+    y.dist_sum = take(y.dist_parts * a.heads * span);
+    if (y.slots * y.splits <= kMaxDistParts) {  // few enough for the last kernel alone
+      y.dist_sum = y.dist;
+      y.dist_parts = (int)(y.slots * y.splits);
+    }
   }
+  if (x.splits > 1) x.part_delta = take((int64_t)x.splits * a.heads * a.nq);
+  // dQ's parts are added up before dK's and dV's come into the same place
+  const int64_t of_q = x.splits > 1 ? (int64_t)x.splits * a.nq * a.heads * a.dim : 0;
+  const int64_t of_k = y.splits > 1 ? 2LL * y.splits * a.nk * a.kv_heads * a.dim : 0;
+  x.part_o = y.part_o = take(std::max(of_q, of_k));
   return bytes;
 }
 
@@ -219,8 +262,8 @@ int ixh_attend_workspace(const ixh_attend_args *a, int backward, int64_t *bytes)
   AttendArgs x{};
   x.a = *a;
   fill_in(x.a);
-  int64_t key_slots;
-  *bytes = backward ? plan_backward(x, &key_slots) : plan_forward(x).work;
+  AttendArgs y;
+  *bytes = backward ? plan_backward(x, y) : plan_forward(x).work;
   return IXH_OK;
 }
 
@@ -267,36 +310,32 @@ int ixh_attend_backward(int device, const ixh_attend_args *a, const ixh_attend_g
         (rc = check_heads("AttendBackward", "dv", g->dv, a->type)))
       return rc;
   }
-  int64_t key_slots;
-  const int64_t need = plan_backward(x, &key_slots);
-  if (x.slots * a->heads > kMaxGrid || key_slots * a->kv_heads > kMaxGrid)
+  AttendArgs y;
+  const int64_t need = plan_backward(x, y);
+  if (x.slots * a->heads > kMaxGrid || y.slots * a->kv_heads > kMaxGrid)
     return fail(IXH_EINVAL, "linalg: AttendBackward: too many rows and heads for one launch");
   if ((rc = check_workspace("AttendBackward", a->workspace, a->workspace_bytes, need))) return rc;
   OnDevice on(device);
   if (on.err != hipSuccess) return hip_fail(on.err, "hipSetDevice");
   hipStream_t const st = (hipStream_t)stream;
-  char *w = (char *)a->workspace;
-  x.delta = (float *)w;
-  AttendArgs y = x;
-  y.slots = key_slots;
-  if (g->dtable) {
-    const int64_t span = 2LL * a->reach + 1;
-    w += up(4LL * a->heads * a->nq);
-    y.dist = (float *)w;
-    y.dist_sum = (float *)(w + up(4 * key_slots * a->heads * span));
-    if (key_slots <= kMaxDistParts) {  // few enough for the last kernel alone
-      y.dist_sum = y.dist;
-      y.dist_parts = (int)key_slots;
-    }
-  }
+  if (!g->dtable) y.dist = nullptr;
   if (a->B > 0) {
     if (!launch_attend_dq(x, st)) return fail(IXH_EHIP, "linalg: hip: AttendBackward: LDS refused");
     if ((rc = launched("attend_dq"))) return rc;
+    if (x.splits > 1) {
+      launch_attend_sum(x, false, st);
+      if ((rc = launched("attend_sum"))) return rc;
+    }
     if (!launch_attend_dkv(y, st)) return fail(IXH_EHIP, "linalg: hip: AttendBackward: LDS refused");
     if ((rc = launched("attend_dkv"))) return rc;
+    if (y.splits > 1) {
+      launch_attend_sum(y, true, st);
+      if ((rc = launched("attend_sum"))) return rc;
+    }
   } else {
     y.slots = y.dist_parts = 0;
   }
+  y.slots *= y.splits;
   if (g->dtable) {
     launch_attend_dtable(y, st);
     return launched("attend_dtable");

@@ -36,6 +36,26 @@ __device__ __forceinline__ float shape_scores(v16f &z, float *slope_of, const Sc
   return FEAT & kBias ? 1.0f : sc.gain;
 }
 
+// A block's share of its steps, where they are in parts (blockIdx.y).
+__device__ __forceinline__ void part_of(int splits, int *t_begin, int *t_end) {
+  if (splits == 1) return;
+  const int per = (*t_end - *t_begin + splits - 1) / splits;
+  *t_begin = min(*t_begin + per * (int)blockIdx.y, *t_end);
+  *t_end = min(*t_begin + per, *t_end);
+}
+
+// A lane's columns of one row of a part's sums.
+template <int ND>
+__device__ __forceinline__ void store_part(const v16f *acc, float *to, int dim, int h) {
+#pragma unroll
+  for (int d = 0; d < ND; d++)
+#pragma unroll
+    for (int g = 0; g < 4; g++) {
+      const int c = 32 * d + 8 * g + 4 * h;
+      if (c < dim) *(f4 *)(to + c) = f4{acc[d][4 * g], acc[d][4 * g + 1], acc[d][4 * g + 2], acc[d][4 * g + 3]};
+    }
+}
+
 // ---- dQ ---------------------------------------------------------------------
 
 // As the forward: a lane has a query (row), K and V come through LDS, 32 keys
@@ -92,6 +112,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : DT == 64 ? 3 : 2) void at
     t_begin = l / BK;
     t_end = u >= l ? u / BK + 1 : t_begin;
   }
+  const bool one_step = t_end - t_begin == 1;
+  part_of(x.splits, &t_begin, &t_end);
   const int64_t row = s.q0 + tok;
   const ColumnDocs docs(a.q_docs ? a.q_docs[row] : 0);
 
@@ -134,7 +156,6 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : DT == 64 ? 3 : 2) void at
   if (a.q_docs || (FEAT & kBias)) __syncthreads();
   auto next = [&](int t) { return a.q_docs ? next_live(live, t, t_begin, t_end) : t; };
   float row_sum = 0.0f;  // of dZ
-  const bool one_step = t_end - t_begin == 1;
 
   v16f acc[ND];
 #pragma unroll
@@ -236,6 +257,14 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : DT == 64 ? 3 : 2) void at
   }
 
   row_sum = half_sum(row_sum);
+  if (x.splits > 1) {
+    if (!mine) return;
+    store_part<ND>(acc, x.part_o + (((int64_t)blockIdx.y * a.nq + row) * a.heads + head) * a.dim, a.dim, h);
+    // one step is the first part's, with the delta that it found
+    if (h == 0)
+      x.part_delta[((int64_t)blockIdx.y * a.heads + head) * a.nq + row] = (blockIdx.y == 0 ? delta : 0.0f) + row_sum;
+    return;
+  }
   if (mine && h == 0) x.delta[(int64_t)head * a.nq + row] = delta + row_sum;
   store_rows<T, DT>(acc, a.scale, smem + wave * (32 * DT * (int)sizeof(T)), a.dim, lane, [&](int i) {
     const int r = row0 + wave * 32 + i, tok = token(r);
@@ -293,7 +322,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 || DT == 128 ? 1 : 2) void atte
   const int kvh = blockIdx.x % a.kv_heads;
   int64_t blk;
   const Seq s = find_block(a, true, KEYS, 1, blockIdx.x / a.kv_heads, &blk);
-  const int64_t slot = blockIdx.x / a.kv_heads;
+  const int64_t slot = blockIdx.x / a.kv_heads * x.splits + blockIdx.y;
   if (blk < 0 || blk * KEYS >= s.nk) {
     if (grad_table)
       for (int g = 0; g < x.group; g++)
@@ -318,6 +347,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 || DT == 128 ? 1 : 2) void atte
     t_begin = max(l, 0) / BQ;
     t_end = u >= max(l, 0) ? min(u, s.nq - 1) / BQ + 1 : t_begin;
     if (t_end < t_begin) t_end = t_begin;
+    part_of(x.splits, &t_begin, &t_end);
   }
   const int64_t row = s.k0 + key;
   const ColumnDocs docs(a.k_docs ? a.k_docs[row] : 0);
@@ -587,6 +617,15 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 || DT == 128 ? 1 : 2) void atte
     meet(dk);
     meet(dv);
   }
+  if (x.splits > 1) {
+    int r = first + kw * 32 + (lane & 31);
+    asm volatile("" : "+v"(r));
+    if (qw != 0 || r >= s.nk) return;
+    float *const part = x.part_o + (((int64_t)blockIdx.y * 2 * a.nk + s.k0 + r) * a.kv_heads + kvh) * a.dim;
+    store_part<ND>(dk, part, a.dim, h);
+    store_part<ND>(dv, part + (int64_t)a.nk * a.kv_heads * a.dim, a.dim, h);
+    return;
+  }
   auto to = [&](const ixh_heads &t) {
     return [&, t](int i) {
       const int r = first + kw * 32 + i;
@@ -596,6 +635,33 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 || DT == 128 ? 1 : 2) void atte
   char *const mine_lds = smem + wave * (32 * DT * (int)sizeof(T));
   store_rows<T, DT>(dk, a.scale, mine_lds, a.dim, lane, to(x.g.dk));
   store_rows<T, DT>(dv, 1.0f, mine_lds, a.dim, lane, to(x.g.dv));
+}
+
+// The parts of dQ (and of delta), or of dK and dV (blockIdx.y), in their
+// order: a thread has four columns of a head's row.
+template <class T>
+__global__ __launch_bounds__(64) void attend_sum_kernel(AttendArgs x, bool keys) {
+  const ixh_attend_args &a = x.a;
+  const int quads = a.dim / 4, heads = keys ? a.kv_heads : a.heads, n = keys ? a.nk : a.nq;
+  const int64_t at = (int64_t)blockIdx.x * 64 + threadIdx.x;
+  const int64_t rh = at / quads;
+  const int c = (int)(at - rh * quads) * 4;
+  const int64_t row = rh / heads;
+  const int head = (int)(rh - row * heads);
+  const int *const offs = keys ? a.k_offs : a.q_offs;
+  if (row >= row_at(offs, a.B, n) || row < row_at(offs, 0, n)) return;
+  const int64_t step = (int64_t)n * heads * a.dim;
+  const float *const p = x.part_o + blockIdx.y * step + rh * a.dim + c;
+  f4 v{};
+#pragma unroll 8
+  for (int i = 0; i < x.splits; i++) v += *(const f4 *)(p + i * step * (keys ? 2 : 1));
+  const ixh_heads &to = !keys ? x.g.dq : blockIdx.y ? x.g.dv : x.g.dk;
+  store4((T *)to.p + row * to.row + head * to.head + c, v * (blockIdx.y ? 1.0f : a.scale));
+  if (!keys && c == 0) {
+    float delta = 0.0f;
+    for (int i = 0; i < x.splits; i++) delta += x.part_delta[((int64_t)i * heads + head) * n + row];
+    x.delta[(int64_t)head * n + row] = delta;
+  }
 }
 
 // ---- the table's gradient ----------------------------------------------------
@@ -660,7 +726,8 @@ bool run_dq(const AttendArgs &x, hipStream_t s) {
   const int shm = Sh::BIAS + 4 * x.pack * len;
   static PerDevice lds;
   if (!lds_granted(lds, (const void *)attend_dq_kernel<T, DT, FEAT>, 160 << 10)) return false;
-  attend_dq_kernel<T, DT, FEAT><<<dim3((unsigned)(x.slots * (x.pack > 1 ? x.a.kv_heads : x.a.heads))), Sh::THREADS, shm, s>>>(x);
+  const dim3 grid((unsigned)(x.slots * (x.pack > 1 ? x.a.kv_heads : x.a.heads)), x.splits);
+  attend_dq_kernel<T, DT, FEAT><<<grid, Sh::THREADS, shm, s>>>(x);
   return true;
 }
 template <class T, int DT, int FEAT, int SHARE>
@@ -670,7 +737,7 @@ bool run_dkv_shared(const AttendArgs &x, hipStream_t s) {
   const int shm = Sh::BIAS + 4 * len * (2 + Sh::WAVES);
   static PerDevice lds;
   if (!lds_granted(lds, (const void *)attend_dkv_kernel<T, DT, FEAT, SHARE>, 160 << 10)) return false;
-  attend_dkv_kernel<T, DT, FEAT, SHARE><<<dim3((unsigned)(x.slots * x.a.kv_heads)), Sh::THREADS, shm, s>>>(x);
+  attend_dkv_kernel<T, DT, FEAT, SHARE><<<dim3((unsigned)(x.slots * x.a.kv_heads), x.splits), Sh::THREADS, shm, s>>>(x);
   return true;
 }
 template <class T, int DT, int FEAT>
@@ -706,6 +773,16 @@ bool by_type(const AttendArgs &x, bool dq, hipStream_t s) {
 
 bool launch_attend_dq(const AttendArgs &x, hipStream_t s) { return by_type(x, true, s); }
 bool launch_attend_dkv(const AttendArgs &x, hipStream_t s) { return by_type(x, false, s); }
+
+void launch_attend_sum(const AttendArgs &x, bool keys, hipStream_t s) {
+  const int64_t n = (int64_t)(keys ? x.a.nk : x.a.nq) * (keys ? x.a.kv_heads : x.a.heads) * (x.a.dim / 4);
+  const dim3 grid((unsigned)((n + 63) / 64), keys ? 2 : 1);
+  switch (x.a.type) {
+    case IXH_TYPE_F32: attend_sum_kernel<float><<<grid, 64, 0, s>>>(x, keys); break;
+    case IXH_TYPE_BF16: attend_sum_kernel<__bf16><<<grid, 64, 0, s>>>(x, keys); break;
+    default: attend_sum_kernel<_Float16><<<grid, 64, 0, s>>>(x, keys); break;
+  }
+}
 
 void launch_attend_dtable(const AttendArgs &x, hipStream_t s) {
   const int span = 2 * x.a.reach + 1;

@@ -201,6 +201,36 @@ def test_keys_past_two_workgroups_a_cu(t, name, heads, copies):
 
 
 @pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("dim", [64, 128, 40])
+@pytest.mark.parametrize("name", ["plain", "all", "prefix", "documents", "other_keys"])
+def test_gradients_of_few_long_sequences(t, dim, name):
+    """Few blocks of keys and queries, in parts that are added up; beside a
+    long sequence one of a single step and one row."""
+    rng = np.random.default_rng(23)
+    lens, k_lens, kw = [2010, 30, 1], None, {}
+    if t != "f32":
+        lens = [2010, 30]
+    n = sum(lens)
+    if name == "all":
+        kw.update(cap=4.0, slopes=ref.alibi(2), table=rng.standard_normal((8, 2)), buckets=np.arange(-20, 21) % 8,
+                  causal=True, window=700)
+    if name == "prefix":
+        kw.update(causal=True, prefix=np.array([900, 3, 0][:len(lens)]))
+    if name == "documents":
+        docs = np.sort(rng.integers(0, 3, n))
+        docs[1990:2010] = -1
+        kw["docs"] = docs
+    if name == "other_keys":
+        k_lens = [800, 1300, 0][:len(lens)]
+        kw["causal"] = True
+    seed = np.random.default_rng(24)
+    first = check(seed, t, lens, k_lens, heads=2, kv_heads=1, dim=dim, **kw)
+    again = check(np.random.default_rng(24), t, lens, k_lens, heads=2, kv_heads=1, dim=dim, **kw)
+    for out in first:
+        assert first[out] is None or torch.equal(first[out], again[out]), out
+
+
+@pytest.mark.parametrize("t", TYPES)
 @pytest.mark.parametrize("heads,kv_heads,dim", [(4, 4, 64), (8, 2, 128), (8, 1, 72), (40, 1, 64)])
 def test_one_token(t, heads, kv_heads, dim):
     """A single new query over all its keys: with and without shared key
