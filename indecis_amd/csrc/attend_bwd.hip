@@ -62,7 +62,7 @@ __device__ __forceinline__ void store_part(const v16f *acc, float *to, int dim, 
 // a step. S^T, dP^T and dQ (twice, for dS in two pieces) are its products.
 // Bound by the issue of vector and matrix instructions (8 sequences of 2,048,
 // 16/4 heads of 128, bf16, documents, causal, cap: 245-260 us; 48 sequences of
-// 64-512, 12 heads of 64, learned bias: 75 us).
+// 64-512, 12 heads of 64, learned bias: 78 us).
 
 template <class T, int DT>
 struct DqShape {
@@ -286,7 +286,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : DT == 64 ? 3 : 2) void at
 // (about 2.7 us a step of 64 queries): that, not a rate, is what bounds it (8
 // sequences of 2,048, 16/4 heads of 128, bf16, documents, causal, cap: 410-430
 // us; 48 sequences of 64-512, 12 heads of 64, learned bias with its gradient:
-// 118 us; 24 of 33-300, 6 heads of 48, float32: 67).
+// 122 us; 24 of 33-300, 6 heads of 48, float32: 69).
 template <class T, int DT, int SHARE>
 struct DkvShape {
   static constexpr int WAVES = 4, THREADS = 256, KEYS = 128 / SHARE;

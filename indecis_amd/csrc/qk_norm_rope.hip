@@ -262,7 +262,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 3 : 2) void norm_rope_ba
 }
 
 // A block has 4 columns of one gamma, a thread every 256th part of them.
-// Bound by latency (512 workgroups' parts of 128 columns: 6 us).
+// Bound by latency (512 workgroups' parts of 128 columns: 5 us).
 __global__ __launch_bounds__(256) void norm_rope_gamma_kernel(NormRopeArgs x, int parts) {
   __shared__ f4 strand[4];
   const ixh_norm_rope_args &a = x.a;
