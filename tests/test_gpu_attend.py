@@ -365,6 +365,38 @@ def test_captured_steps_replay():
                 assert (a is None and b is None) or torch.equal(a, b), f"replay {step}"
 
 
+def test_steps_in_parts_captured_and_at_once():
+    """Few long sequences, whose gradients come in parts: two graphs replayed
+    on streams of their own at once, with eager calls between."""
+    rng = np.random.default_rng(25)
+    offs = ints([0, 1700, 2400])
+    sets = [[rows(rng, torch.bfloat16, 2400, h, 64) for h in (4, 2, 2, 4)] for _ in range(2)]
+    kw = dict(causal=True, table=rows(rng, torch.bfloat16, 8, 4), buckets=ints(np.arange(-30, 31) % 8))
+    streams = [torch.cuda.Stream() for _ in sets]
+    graphs = []
+    for st, ts in zip(streams, sets):
+        st.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(st):
+            _training(ts, offs, kw)
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = _training(ts, offs, kw)
+        graphs.append((g, out))
+    for step in range(3):
+        for ts in sets:
+            for x in ts:
+                x.copy_(rows(rng, torch.bfloat16, *x.shape))
+        torch.cuda.synchronize()
+        for st, (g, _) in zip(streams, graphs):
+            with torch.cuda.stream(st):
+                g.replay()
+        torch.cuda.synchronize()
+        for ts, (_, out) in zip(sets, graphs):
+            for a, b in zip(out, _training(ts, offs, kw)):
+                assert torch.equal(a, b), f"replay {step}"
+
+
 def test_streams_at_once():
     """Two calls at once on streams of their own, neither the default."""
     rng = np.random.default_rng(24)
